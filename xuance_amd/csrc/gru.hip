@@ -10,7 +10,7 @@
 // steps) that chain is latency-bound, not throughput-bound, so the recurrence runs ONE WAVEFRONT PER SEQUENCE with no
 // workgroup barrier and no cross-wave traffic at all: lane j owns hidden unit j and keeps its three rows of W_hh (forward)
 // or its column of W_hh (backward) in 192 registers for the whole sequence; the previous hidden state (forward) or the
-// gate gradients (backward) are broadcast to the wave through 256 / 768 bytes of LDS.  A step costs 96 v_pk_fma_f32 per
+// gate gradients (backward) are broadcast to the wave through 256 / 768 bytes of LDS.  A step costs 192 v_fma_f32 per
 // lane + 16 (48) broadcast ds_read_b128; a 32-row MFMA tile would need 6 output tiles x 32 chained v_mfma_f32_32x32x2 per
 // step on one CU and leave all but 3 CUs idle.  Per-step operands that do not depend on the recurrence (gi; saved gates
 // and d_hs in the backward pass) are loaded two steps ahead into a statically indexed 3-slot register ring, so no step
@@ -22,7 +22,7 @@ namespace xrl {
 constexpr int GH = 64;    // hidden width == wavefront width
 
 typedef float v2f __attribute__((ext_vector_type(2)));
-// two fp32 FMAs per lane and issue slot (v_pk_fma_f32): the dot products run as two half-sums (k < 32 | k >= 32)
+// the dot products run as two half-sums (k < 32 | k >= 32), one pair of fp32 FMAs at a time
 __device__ __forceinline__ v2f pk_fma(v2f a, v2f b, v2f c) { return __builtin_elementwise_fma(a, b, c); }
 
 // v_exp_f32 / v_rcp_f32 (1 ulp each) instead of the branchy libm expf / tanhf / IEEE division: the gate non-linearities sit

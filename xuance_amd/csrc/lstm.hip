@@ -4,7 +4,7 @@
 //   i = sigmoid(.)  f = sigmoid(.)  g = tanh(.)  o = sigmoid(.)   of   gi + W_hh h + b_hh;   c' = f c + i g;   h' = o tanh(c')
 // Same mapping as csrc/gru.hip (see there): the input-side products and every weight gradient are chip-wide GEMMs; the
 // recurrence runs one two-wave workgroup per sequence, lane j = hidden unit j, each wave holding half of unit j's four
-// W_hh rows (forward) / half of column j (backward) in 128 registers, packed fp32 FMAs, operands that do not depend on
+// W_hh rows (forward) / half of column j (backward) in 128 registers, paired fp32 FMAs, operands that do not depend on
 // the recurrence prefetched two steps ahead.  The gate pre-activation gradient is the same for the input and the hidden
 // side, so the backward pass writes one d_gates buffer (dW_ih = d_gates^T x, dW_hh = d_gates^T h_prev).
 #include "common.h"
