@@ -1516,6 +1516,95 @@ int xrl_per_update_priorities(double* sum_tree, double* min_tree, double* max_pr
                               const float* priorities, double alpha, int n_envs, int capacity, int per_env,
                               xrl_stream_t stream);
 
+/* ------------------------------------------------------------------ sequence policies (no counterpart in the reference)
+ * Storage type of the activations of the entry points below; parameters, states, sums and statistics are always f32. */
+enum { XRL_F32 = 0, XRL_BF16 = 1 };
+
+/* Linear attention with one decay per head: the sequence core next to the GRU / LSTM above.  For row b and head h
+ *     S_t = lam_h S_{t-1} + k_t (x) v_t        (reset[t][b] != 0: S_{t-1} := 0 first)        o_t = scale * q_t S_t
+ * with lam_h = exp(log_decay[h]), log_decay <= 0 (-inf: no memory).  Positive values are taken as 0.  S is [dk][dv], f32.
+ * Activations are [T][B][H][d] with any strides over T, B and H (elements, 64 bits; d contiguous): stride_*[0] = from step to step,
+ * [1] = from row to row, [2] = from head to head.  Stride 0 shares an input among heads or rows; outputs need every element of their own
+ * and overlap no input.  lengths: steps at and behind lengths[b] are not read, take no part and their outputs are written as 0;
+ * state_out is S after step lengths[b] - 1.  Inputs have to be finite: a NaN or infinity reaches the 64 steps around its own. */
+typedef struct {
+    const void* q;           /* [T][B][H][dk] */
+    const void* k;           /* [T][B][H][dk] */
+    const void* v;           /* [T][B][H][dv] */
+    void* out;               /* forward, step: [T][B][H][dv] */
+    const float* log_decay;  /* [H] */
+    const int32_t* lengths;  /* NULL (all T) or [B], taken into 0..T; not used by the step */
+    const float* reset;      /* NULL or [T][B] contiguous */
+    const float* state;      /* NULL (zeros; the step needs it) or [B][H][dk][dv]: S before the first step */
+    float* state_out;        /* NULL (the step needs it) or [B][H][dk][dv]: S after the last step; may be `state` itself */
+    const void* d_out;       /* backward: [T][B][H][dv] */
+    void* d_q; void* d_k; void* d_v;
+    const float* d_state_out;  /* NULL (zeros) or [B][H][dk][dv]: gradient of state_out */
+    float* d_state;          /* NULL or [B][H][dk][dv]: gradient of state; not d_state_out itself */
+    float* workspace;        /* xrl_linattn_workspace_floats() floats, 16-byte aligned; contents need not survive the call */
+    int64_t workspace_floats;
+    int64_t stride_q[3], stride_k[3], stride_v[3], stride_out[3], stride_d_out[3], stride_d_q[3], stride_d_k[3], stride_d_v[3];
+    int32_t T, B, H, dk, dv; /* dk, dv in 1..128 */
+    int32_t dtype;           /* XRL_F32, XRL_BF16: q k v out and their gradients */
+    float scale; int32_t pad;
+} xrl_linattn_t;
+/* floats of workspace that the forward (backward = 0) or backward (1) pass over these sizes needs; 0: none */
+int64_t xrl_linattn_workspace_floats(const xrl_linattn_t* p, int backward);
+int xrl_linattn_forward(const xrl_linattn_t* p, xrl_stream_t stream);
+/* d_q, d_k, d_v and (where asked for) d_state from d_out and d_state_out.  log_decay is a constant of the head: it has no gradient. */
+int xrl_linattn_backward(const xrl_linattn_t* p, xrl_stream_t stream);
+/* One acting step: T must be 1, reset is [B]. */
+int xrl_linattn_step(const xrl_linattn_t* p, xrl_stream_t stream);
+
+/* The norms before and after a residual block, with the block's gate and residual scale, over rows of D values:
+ *     p = norm(u) * w_post + b_post        y = x + scale * act(gate) * p        n = norm(y) * w_pre + b_pre
+ * u = output of the block, x = the residual stream before it, y = the stream after it, n = input of the next block (from the unrounded y).
+ * norm: XRL_NORM_RMS r = 1 / sqrt(mean(a^2) + eps), a r (eps > 0); XRL_NORM_LAYER the same of a - mean(a).
+ * A missing gate, scale or weight is 1, a missing bias 0.  ld_*: elements from row to row.  y may be x, d_x may be d_y. */
+enum { XRL_NORM_RMS = 0, XRL_NORM_LAYER = 1 };
+typedef struct {
+    const void* x; const void* u;          /* [N][D] */
+    const void* gate;                      /* NULL or [N][D], before its activation */
+    void* y; void* n;                      /* forward: [N][D]; n may be NULL */
+    const float* scale;                    /* NULL or [D] */
+    const float* w_post; const float* b_post; const float* w_pre; const float* b_pre;   /* NULL or [D] */
+    const void* d_y; const void* d_n;      /* backward: [N][D], either may be NULL (zeros) */
+    void* d_x; void* d_u;                  /* backward: [N][D] */
+    void* d_gate;                          /* NULL or [N][D] */
+    float* d_scale; float* d_w_post; float* d_b_post; float* d_w_pre; float* d_b_pre;   /* NULL or [D]: sums over the rows */
+    float* workspace;                      /* backward: xrl_block_norm_workspace_floats() floats; contents need not survive the call */
+    int64_t workspace_floats;
+    int64_t N;
+    int64_t ld_x, ld_u, ld_gate, ld_y, ld_n, ld_d_y, ld_d_n, ld_d_x, ld_d_u, ld_d_gate;
+    int32_t D;                             /* 1..8192 */
+    int32_t dtype, kind, gate_act;         /* gate_act: XRL_ACT_* */
+    float eps; int32_t pad;
+} xrl_block_norm_t;
+int64_t xrl_block_norm_workspace_floats(const xrl_block_norm_t* p);
+int xrl_block_norm_forward(const xrl_block_norm_t* p, xrl_stream_t stream);
+int xrl_block_norm_backward(const xrl_block_norm_t* p, xrl_stream_t stream);
+
+/* Distillation of a categorical policy from a teacher's top logits, with its gradient, in one launch.  Per row n
+ *     q = softmax(teacher_logits / tau) over the row's valid entries      p = softmax(logits / tau) over the available actions
+ *     loss = weight tau^2 sum_k q_k (log q_k - log p_{teacher_idx_k})     d_logits_a = grad_scale weight tau (p_a - q_a)
+ * An entry is valid if its index is in 0..A-1, its action available and its logit above -inf; the same action named twice counts twice.
+ * Unavailable actions get gradient 0 and their logits are not used.  A row without a valid entry, without an available logit above -inf,
+ * or with weight 0 has loss 0 and gradient 0, whatever its logits hold. */
+typedef struct {
+    const void* logits;            /* [N][ld] */
+    const int32_t* teacher_idx;    /* [N][K] */
+    const void* teacher_logits;    /* [N][K], type of logits */
+    const float* avail;            /* NULL or [N][A] f32 0/1 */
+    const float* weight;           /* NULL (1) or [N] */
+    float* loss;                   /* [N] */
+    void* d_logits;                /* NULL (loss only) or [N][ld_d]; may be `logits` itself */
+    int64_t N, ld, ld_d;
+    int32_t A, K;                  /* K in 1..256 */
+    int32_t dtype;
+    float temperature, grad_scale; int32_t pad;
+} xrl_distill_t;
+int xrl_distill_loss(const xrl_distill_t* p, xrl_stream_t stream);
+
 /* Hard target update inside a captured graph: if (state->step % sync_frequency == 0) target <- params
  * (dqn_learner.py:56-57, qmix_learner.py:105-106; copy_target deep_q_network.py:95-99). */
 int xrl_sync_target(const float* params, float* target, int64_t P, const xrl_adam_state_t* state,

@@ -389,7 +389,37 @@ class MarlAct(C.Structure):
                 ("eps", c_float), ("seed", C.c_uint64), ("step", C.c_uint32), ("step_dev", c_void_p)]
 
 
+class LinAttn(C.Structure):
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("out", c_void_p), ("log_decay", c_void_p), ("lengths", c_void_p),
+                ("reset", c_void_p), ("state", c_void_p), ("state_out", c_void_p), ("d_out", c_void_p), ("d_q", c_void_p), ("d_k", c_void_p),
+                ("d_v", c_void_p), ("d_state_out", c_void_p), ("d_state", c_void_p), ("workspace", c_void_p), ("workspace_floats", c_int64),
+                ("stride_q", c_int64 * 3), ("stride_k", c_int64 * 3), ("stride_v", c_int64 * 3), ("stride_out", c_int64 * 3),
+                ("stride_d_out", c_int64 * 3), ("stride_d_q", c_int64 * 3), ("stride_d_k", c_int64 * 3), ("stride_d_v", c_int64 * 3),
+                ("T", c_int32), ("B", c_int32), ("H", c_int32), ("dk", c_int32), ("dv", c_int32), ("dtype", c_int32),
+                ("scale", c_float), ("pad", c_int32)]
+
+
+class BlockNorm(C.Structure):
+    _fields_ = [(f, c_void_p) for f in ("x", "u", "gate", "y", "n", "scale", "w_post", "b_post", "w_pre", "b_pre", "d_y", "d_n", "d_x", "d_u",
+                                        "d_gate", "d_scale", "d_w_post", "d_b_post", "d_w_pre", "d_b_pre", "workspace")] + \
+               [(f, c_int64) for f in ("workspace_floats", "N", "ld_x", "ld_u", "ld_gate", "ld_y", "ld_n", "ld_d_y", "ld_d_n", "ld_d_x", "ld_d_u",
+                                       "ld_d_gate")] + \
+               [("D", c_int32), ("dtype", c_int32), ("kind", c_int32), ("gate_act", c_int32), ("eps", c_float), ("pad", c_int32)]
+
+
+class Distill(C.Structure):
+    _fields_ = [("logits", c_void_p), ("teacher_idx", c_void_p), ("teacher_logits", c_void_p), ("avail", c_void_p), ("weight", c_void_p),
+                ("loss", c_void_p), ("d_logits", c_void_p), ("N", c_int64), ("ld", c_int64), ("ld_d", c_int64), ("A", c_int32), ("K", c_int32),
+                ("dtype", c_int32), ("temperature", c_float), ("grad_scale", c_float), ("pad", c_int32)]
+
+
 _SIGS = {
+    "xrl_linattn_forward": [C.POINTER(LinAttn), c_void_p],
+    "xrl_linattn_backward": [C.POINTER(LinAttn), c_void_p],
+    "xrl_linattn_step": [C.POINTER(LinAttn), c_void_p],
+    "xrl_block_norm_forward": [C.POINTER(BlockNorm), c_void_p],
+    "xrl_block_norm_backward": [C.POINTER(BlockNorm), c_void_p],
+    "xrl_distill_loss": [C.POINTER(Distill), c_void_p],
     "xrl_marl_select_actions": [C.POINTER(MarlAct), c_void_p],
     "xrl_ppo_fused_minibatch": [C.POINTER(PpoFused), c_void_p],
     "xrl_ppo_trunk_chained": [C.POINTER(PpoFused), C.POINTER(OptChain), c_void_p],
@@ -529,7 +559,8 @@ _lib = None
 
 def exported_symbols():
     """Names every entry point include/xrl_hip.h declares (checked by the CPU test-suite)."""
-    return ["xrl_version", "xrl_last_error", "xrl_rollout_cache_floats", "xrl_rollout_wide_words"] + list(_SIGS)
+    return ["xrl_version", "xrl_last_error", "xrl_rollout_cache_floats", "xrl_rollout_wide_words", "xrl_linattn_workspace_floats",
+            "xrl_block_norm_workspace_floats"] + list(_SIGS)
 
 
 def load():
@@ -550,6 +581,10 @@ def load():
     lib.xrl_rollout_cache_floats.argtypes = [C.POINTER(RolloutStep)]
     lib.xrl_rollout_wide_words.restype = c_int
     lib.xrl_rollout_wide_words.argtypes = []
+    lib.xrl_linattn_workspace_floats.restype = c_int64
+    lib.xrl_linattn_workspace_floats.argtypes = [C.POINTER(LinAttn), c_int]
+    lib.xrl_block_norm_workspace_floats.restype = c_int64
+    lib.xrl_block_norm_workspace_floats.argtypes = [C.POINTER(BlockNorm)]
     for name, args in _SIGS.items():
         fn = getattr(lib, name)
         fn.argtypes = args

@@ -1,0 +1,399 @@
+// The norms before and after a residual block, fused with the block's gate and residual scale (include/xrl_hip.h: xrl_block_norm_*).
+//
+//     p = norm(u) w_post + b_post,   y = x + scale act(gate) p,   n = norm(y) w_pre + b_pre
+//
+// Bound by memory: forward 3 reads + 2 writes, backward 5 reads + 3 writes of N x D values and nothing saved in between -- the backward
+// pass recomputes p, y and both statistics from the x, u and gate it needs anyway.  A row lives in the registers of L lanes, 8 values
+// each, from its one load to its one store; the parameters and the gradient sums over the rows stay in registers over all rows of a
+// workgroup.  Those sums leave as one line of partials per workgroup and a second launch adds the lines in a fixed order (no atomics).
+#include "io16.h"
+
+namespace xrl {
+
+constexpr int NV = 8;                  // values of a row per lane
+constexpr int NORM_SUMS = 5;           // d_scale, d_w_post, d_b_post, d_w_pre, d_b_pre
+
+template <int L>
+struct norm_geom {
+    static constexpr int THREADS = L < 256 ? (L > 64 ? L : 256) : L;
+    static constexpr int ROWS = L > 64 ? 1 : THREADS / L;        // rows of a workgroup at a time
+    static constexpr int WAVES = THREADS / 64;
+};
+
+// lane's m-th value of a row: 8 neighbours where the rows allow 16-byte accesses, else one every L
+template <int L, bool VEC>
+__device__ __forceinline__ int norm_at(int lane, int m) { return VEC ? lane * NV + m : lane + L * m; }
+
+template <typename E, int L, bool VEC>
+__device__ __forceinline__ void norm_load(const E* row, int lane, int D, float (&v)[NV]) {
+    if (VEC) {
+#pragma unroll
+        for (int m = 0; m < NV; ++m) v[m] = 0.f;
+        if (lane * NV < D) {
+            if (sizeof(E) == 4) {
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    const f32x4_t x = reinterpret_cast<const f32x4_t*>(row)[lane * 2 + q];
+#pragma unroll
+                    for (int m = 0; m < 4; ++m) v[4 * q + m] = x[m];
+                }
+            } else {
+                const u32x4_t x = reinterpret_cast<const u32x4_t*>(row)[lane];
+#pragma unroll
+                for (int m = 0; m < 4; ++m) { v[2 * m] = __uint_as_float(x[m] << 16); v[2 * m + 1] = __uint_as_float(x[m] & 0xffff0000u); }
+            }
+        }
+    } else {
+#pragma unroll
+        for (int m = 0; m < NV; ++m) v[m] = lane + L * m < D ? io_load(row + lane + L * m) : 0.f;
+    }
+}
+
+template <typename E, int L, bool VEC>
+__device__ __forceinline__ void norm_store(E* row, int lane, int D, const float (&v)[NV]) {
+    if (VEC) {
+        if (lane * NV < D) {
+            if (sizeof(E) == 4) {
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    const f32x4_t x = {v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+                    reinterpret_cast<f32x4_t*>(row)[lane * 2 + q] = x;
+                }
+            } else {
+                const u32x4_t x = {cvt_pk_bf16(v[0], v[1]), cvt_pk_bf16(v[2], v[3]), cvt_pk_bf16(v[4], v[5]), cvt_pk_bf16(v[6], v[7])};
+                reinterpret_cast<u32x4_t*>(row)[lane] = x;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int m = 0; m < NV; ++m)
+            if (lane + L * m < D) io_store(row + lane + L * m, v[m]);
+    }
+}
+
+template <int L, bool VEC>
+__device__ __forceinline__ void norm_param(const float* p, int lane, int D, float missing, float (&v)[NV]) {
+#pragma unroll
+    for (int m = 0; m < NV; ++m) {
+        const int e = norm_at<L, VEC>(lane, m);
+        v[m] = e < D ? (p ? p[e] : missing) : 0.f;
+    }
+}
+
+// Sums over the L lanes of a row.  Across waves through LDS with one barrier: consecutive sums use other slots of `scratch`, and a slot
+// comes round again only two barriers later.
+template <int L>
+struct row_sum_t {
+    float2 (*scratch)[16];
+    int slot;
+    __device__ __forceinline__ float2 operator()(float a, float b) {
+#pragma unroll
+        for (int off = (L < 64 ? L : 64) / 2; off > 0; off >>= 1) { a += __shfl_xor(a, off, 64); b += __shfl_xor(b, off, 64); }
+        if (L > 64) {
+            const int w = threadIdx.x >> 6;
+            slot = slot == 2 ? 0 : slot + 1;
+            if ((threadIdx.x & 63) == 0) scratch[slot][w] = make_float2(a, b);
+            __syncthreads();
+            a = b = 0.f;
+#pragma unroll
+            for (int i = 0; i < L / 64; ++i) { a += scratch[slot][i].x; b += scratch[slot][i].y; }
+        }
+        return make_float2(a, b);
+    }
+    __device__ __forceinline__ float operator()(float a) {
+#pragma unroll
+        for (int off = (L < 64 ? L : 64) / 2; off > 0; off >>= 1) a += __shfl_xor(a, off, 64);
+        if (L > 64) {
+            const int w = threadIdx.x >> 6;
+            slot = slot == 2 ? 0 : slot + 1;
+            if ((threadIdx.x & 63) == 0) scratch[slot][w].x = a;
+            __syncthreads();
+            a = 0.f;
+#pragma unroll
+            for (int i = 0; i < L / 64; ++i) a += scratch[slot][i].x;
+        }
+        return a;
+    }
+};
+
+// v := (v - mean) r (layer) or v r; returns r.  The variance is taken of the centred values (no difference of large sums).
+template <int L, bool VEC, bool LN>
+__device__ __forceinline__ float normalize(float (&v)[NV], int lane, int D, float inv_d, float eps, row_sum_t<L>& sum) {
+    if (LN) {
+        float s = 0.f;
+#pragma unroll
+        for (int m = 0; m < NV; ++m) s += v[m];
+        const float mean = sum(s) * inv_d;
+#pragma unroll
+        for (int m = 0; m < NV; ++m) v[m] = norm_at<L, VEC>(lane, m) < D ? v[m] - mean : 0.f;
+    }
+    float q = 0.f;
+#pragma unroll
+    for (int m = 0; m < NV; ++m) q += v[m] * v[m];
+    const float r = 1.f / sqrtf(sum(q) * inv_d + eps);
+#pragma unroll
+    for (int m = 0; m < NV; ++m) v[m] *= r;
+    return r;
+}
+
+template <typename E, int L, bool VEC, bool LN>
+__global__ void __launch_bounds__(norm_geom<L>::THREADS) block_norm_fwd_kernel(xrl_block_norm_t p) {
+    using G = norm_geom<L>;
+    __shared__ float2 scratch[3][16];
+    row_sum_t<L> sum{scratch, 0};
+    const int lane = threadIdx.x % L, D = p.D;
+    const float inv_d = 1.f / (float)D;
+    float sc[NV], w0[NV], b0[NV], w1[NV], b1[NV];
+    norm_param<L, VEC>(p.scale, lane, D, 1.f, sc);
+    norm_param<L, VEC>(p.w_post, lane, D, 1.f, w0);
+    norm_param<L, VEC>(p.b_post, lane, D, 0.f, b0);
+    norm_param<L, VEC>(p.w_pre, lane, D, 1.f, w1);
+    norm_param<L, VEC>(p.b_pre, lane, D, 0.f, b1);
+    const int64_t step = (int64_t)gridDim.x * G::ROWS;
+    for (int64_t base = (int64_t)blockIdx.x * G::ROWS; base < p.N; base += step) {       // whole workgroups go round: barriers inside
+        const int64_t row = base + threadIdx.x / L;
+        const bool live = row < p.N;
+        float x[NV] = {}, u[NV] = {}, g[NV] = {};
+        if (live) {
+            norm_load<E, L, VEC>((const E*)p.u + row * p.ld_u, lane, D, u);
+            norm_load<E, L, VEC>((const E*)p.x + row * p.ld_x, lane, D, x);
+            if (p.gate) norm_load<E, L, VEC>((const E*)p.gate + row * p.ld_gate, lane, D, g);
+        }
+        normalize<L, VEC, LN>(u, lane, D, inv_d, p.eps, sum);
+        if (p.gate) {
+            XRL_ACT_DISPATCH(p.gate_act, _Pragma("unroll") for (int m = 0; m < NV; ++m) g[m] = act_apply_c<ACT>(g[m]);)
+        }
+#pragma unroll
+        for (int m = 0; m < NV; ++m) {
+            const float b = sc[m] * (u[m] * w0[m] + b0[m]);
+            x[m] += p.gate ? g[m] * b : b;
+        }
+        if (live) norm_store<E, L, VEC>((E*)p.y + row * p.ld_y, lane, D, x);
+        if (p.n) {
+            normalize<L, VEC, LN>(x, lane, D, inv_d, p.eps, sum);
+#pragma unroll
+            for (int m = 0; m < NV; ++m) x[m] = x[m] * w1[m] + b1[m];
+            if (live) norm_store<E, L, VEC>((E*)p.n + row * p.ld_n, lane, D, x);
+        }
+    }
+}
+
+// d := r (d - xhat mean(d xhat) [- mean(d)]): gradient through the normalisation
+template <int L, bool VEC, bool LN>
+__device__ __forceinline__ void normalize_back(float (&d)[NV], const float (&xhat)[NV], float r, int lane, int D, float inv_d,
+                                               row_sum_t<L>& sum) {
+    float a = 0.f, b = 0.f;
+#pragma unroll
+    for (int m = 0; m < NV; ++m) { a += d[m] * xhat[m]; if (LN) b += d[m]; }
+    if (LN) { const float2 t = sum(a, b); a = t.x * inv_d; b = t.y * inv_d; }
+    else a = sum(a) * inv_d;
+#pragma unroll
+    for (int m = 0; m < NV; ++m) d[m] = norm_at<L, VEC>(lane, m) < D ? r * (d[m] - xhat[m] * a - b) : 0.f;
+}
+
+template <typename E, int L, bool VEC, bool LN>
+__global__ void __launch_bounds__(norm_geom<L>::THREADS) block_norm_bwd_kernel(xrl_block_norm_t p) {
+    using G = norm_geom<L>;
+    __shared__ float2 scratch[3][16];
+    row_sum_t<L> sum{scratch, 0};
+    const int lane = threadIdx.x % L, D = p.D;
+    const float inv_d = 1.f / (float)D;
+    float sc[NV], w0[NV], b0[NV], w1[NV];
+    norm_param<L, VEC>(p.scale, lane, D, 1.f, sc);
+    norm_param<L, VEC>(p.w_post, lane, D, 1.f, w0);
+    norm_param<L, VEC>(p.b_post, lane, D, 0.f, b0);
+    norm_param<L, VEC>(p.w_pre, lane, D, 1.f, w1);
+    float acc[NORM_SUMS][NV] = {};
+    const int64_t step = (int64_t)gridDim.x * G::ROWS;
+    for (int64_t base = (int64_t)blockIdx.x * G::ROWS; base < p.N; base += step) {
+        const int64_t row = base + threadIdx.x / L;
+        const bool live = row < p.N;
+        float x[NV] = {}, u[NV] = {}, g[NV] = {}, dy[NV] = {}, dn[NV] = {}, t[NV];
+        if (live) {
+            norm_load<E, L, VEC>((const E*)p.u + row * p.ld_u, lane, D, u);
+            norm_load<E, L, VEC>((const E*)p.x + row * p.ld_x, lane, D, x);
+            if (p.gate) norm_load<E, L, VEC>((const E*)p.gate + row * p.ld_gate, lane, D, g);
+            if (p.d_y) norm_load<E, L, VEC>((const E*)p.d_y + row * p.ld_d_y, lane, D, dy);
+            if (p.d_n) norm_load<E, L, VEC>((const E*)p.d_n + row * p.ld_d_n, lane, D, dn);
+        }
+        const float ru = normalize<L, VEC, LN>(u, lane, D, inv_d, p.eps, sum);
+        if (p.gate) {
+            XRL_ACT_DISPATCH(p.gate_act, _Pragma("unroll") for (int m = 0; m < NV; ++m) g[m] = act_apply_c<ACT>(g[m]);)
+        }
+        if (p.d_n) {
+#pragma unroll
+            for (int m = 0; m < NV; ++m) {
+                const float b = sc[m] * (u[m] * w0[m] + b0[m]);
+                x[m] += p.gate ? g[m] * b : b;
+            }
+            const float ry = normalize<L, VEC, LN>(x, lane, D, inv_d, p.eps, sum);
+#pragma unroll
+            for (int m = 0; m < NV; ++m) { acc[3][m] += dn[m] * x[m]; acc[4][m] += dn[m]; t[m] = dn[m] * w1[m]; }
+            normalize_back<L, VEC, LN>(t, x, ry, lane, D, inv_d, sum);
+#pragma unroll
+            for (int m = 0; m < NV; ++m) dy[m] += t[m];
+        }
+        if (live) norm_store<E, L, VEC>((E*)p.d_x + row * p.ld_d_x, lane, D, dy);
+        // y = x + scale a p: with a the activated gate
+#pragma unroll
+        for (int m = 0; m < NV; ++m) {
+            const float pm = u[m] * w0[m] + b0[m], da = dy[m] * (p.gate ? g[m] : 1.f), dp = da * sc[m];
+            acc[0][m] += da * pm; acc[1][m] += dp * u[m]; acc[2][m] += dp;
+            t[m] = dp * w0[m];
+            dy[m] *= sc[m] * pm;                                     // gradient of the activated gate
+        }
+        if (p.d_gate) {
+            XRL_ACT_DISPATCH(p.gate_act, _Pragma("unroll") for (int m = 0; m < NV; ++m) g[m] = dy[m] * act_grad_c<ACT>(g[m]);)
+            if (live) norm_store<E, L, VEC>((E*)p.d_gate + row * p.ld_d_gate, lane, D, g);
+        }
+        normalize_back<L, VEC, LN>(t, u, ru, lane, D, inv_d, sum);
+        if (live) norm_store<E, L, VEC>((E*)p.d_u + row * p.ld_d_u, lane, D, t);
+    }
+    // partial sums: over the rows of a wave, then over the waves (in wave order), one line per workgroup
+    float* line = p.workspace + (size_t)blockIdx.x * NORM_SUMS * D;
+    __shared__ float part[L > 64 ? 1 : G::WAVES][L > 64 ? 1 : L * NV];
+#pragma unroll
+    for (int s = 0; s < NORM_SUMS; ++s) {
+        if (L < 64) {
+#pragma unroll
+            for (int off = L; off < 64; off <<= 1)
+#pragma unroll
+                for (int m = 0; m < NV; ++m) acc[s][m] += __shfl_xor(acc[s][m], off, 64);
+        }
+        if (L > 64) {
+#pragma unroll
+            for (int m = 0; m < NV; ++m) {
+                const int e = norm_at<L, VEC>(lane, m);
+                if (e < D) line[s * D + e] = acc[s][m];
+            }
+        } else {
+            __syncthreads();
+            if ((int)(threadIdx.x & 63) < L) {
+#pragma unroll
+                for (int m = 0; m < NV; ++m) part[threadIdx.x >> 6][norm_at<L, VEC>(lane, m)] = acc[s][m];
+            }
+            __syncthreads();
+            for (int e = threadIdx.x; e < D; e += G::THREADS) {
+                float t = 0.f;
+#pragma unroll
+                for (int w = 0; w < G::WAVES; ++w) t += part[w][e];
+                line[s * D + e] = t;
+            }
+        }
+    }
+}
+
+// out[s][e] = sum of the workgroups' lines, 64 groups of lines a column, met in a fixed order
+__global__ void __launch_bounds__(1024) block_norm_sums_kernel(xrl_block_norm_t p, int lines) {
+    __shared__ float part[64][17];
+    const int c = threadIdx.x & 15, r = threadIdx.x >> 4, width = NORM_SUMS * p.D;
+    const int col = blockIdx.x * 16 + c;
+    float t = 0.f;
+    if (col < width)
+        for (int i = r; i < lines; i += 64) t += p.workspace[(size_t)i * width + col];
+    part[r][c] = t;
+    __syncthreads();
+    if (threadIdx.x < 16 && col < width) {
+        float a = 0.f;
+        for (int i = 0; i < 64; ++i) a += part[i][c];
+        float* outs[NORM_SUMS] = {p.d_scale, p.d_w_post, p.d_b_post, p.d_w_pre, p.d_b_pre};
+#pragma unroll
+        for (int s = 0; s < NORM_SUMS; ++s)
+            if (outs[s] && col / p.D == s) outs[s][col % p.D] = a;
+    }
+}
+
+static int norm_lanes(int D) {
+    int L = 8;
+    while (L * NV < D) L *= 2;
+    return L;
+}
+
+// workgroups of the backward pass: enough to fill the chip twice over, each with rows to keep its parameters and sums for
+static int norm_lines(const xrl_block_norm_t& p) {
+    const int L = norm_lanes(p.D), threads = L < 256 ? (L > 64 ? L : 256) : L, rows = L > 64 ? 1 : threads / L;
+    const int64_t most = 512 * 256 / threads, need = (p.N + rows - 1) / rows;
+    return (int)(need < most ? need : most);
+}
+
+static int check_norm(const xrl_block_norm_t& p) {
+    XRL_CHECK_ARG(p.N >= 0 && p.D >= 1 && p.D <= 8192);
+    XRL_CHECK_ARG((p.dtype == XRL_F32 || p.dtype == XRL_BF16) && (p.kind == XRL_NORM_RMS || p.kind == XRL_NORM_LAYER));
+    XRL_CHECK_ARG(p.gate_act >= XRL_ACT_NONE && p.gate_act <= XRL_ACT_SIGMOID && p.eps > 0.f);
+    return XRL_OK;
+}
+
+static bool norm_vec(const xrl_block_norm_t& p, bool backward) {
+    const void* ptr[10] = {p.x, p.u, p.gate, p.y, p.n, p.d_y, p.d_n, p.d_x, p.d_u, p.d_gate};
+    const int64_t ld[10] = {p.ld_x, p.ld_u, p.ld_gate, p.ld_y, p.ld_n, p.ld_d_y, p.ld_d_n, p.ld_d_x, p.ld_d_u, p.ld_d_gate};
+    if (p.D % NV) return false;
+    const int unit = p.dtype == XRL_F32 ? 4 : 8;
+    for (int i = 0; i < 10; ++i) {
+        if (!ptr[i] || (backward ? (i == 3 || i == 4) : i > 4)) continue;
+        if ((reinterpret_cast<uintptr_t>(ptr[i]) & 15) || ld[i] % unit) return false;
+    }
+    return true;
+}
+
+template <typename E, bool VEC, bool LN>
+static void launch_norm(const xrl_block_norm_t& p, bool backward, hipStream_t s) {
+    const int L = norm_lanes(p.D);
+#define NORM_CASE(LL)                                                                                                            \
+    case LL: {                                                                                                                   \
+        using G = norm_geom<LL>;                                                                                                 \
+        if (backward) hipLaunchKernelGGL((block_norm_bwd_kernel<E, LL, VEC, LN>), dim3(norm_lines(p)), dim3(G::THREADS), 0, s, p); \
+        else {                                                                                                                   \
+            const int64_t need = (p.N + G::ROWS - 1) / G::ROWS, most = 2048 * 256 / G::THREADS;                                  \
+            hipLaunchKernelGGL((block_norm_fwd_kernel<E, LL, VEC, LN>), dim3((int)(need < most ? need : most)), dim3(G::THREADS), 0, s, p); \
+        }                                                                                                                        \
+    } break;
+    switch (L) { NORM_CASE(8) NORM_CASE(16) NORM_CASE(32) NORM_CASE(64) NORM_CASE(128) NORM_CASE(256) NORM_CASE(512) NORM_CASE(1024) }
+#undef NORM_CASE
+}
+
+static int run_norm(const xrl_block_norm_t& p, bool backward, hipStream_t s) {
+    const bool vec = norm_vec(p, backward), ln = p.kind == XRL_NORM_LAYER;
+    if (p.dtype == XRL_F32) {
+        if (vec) { if (ln) launch_norm<float, true, true>(p, backward, s); else launch_norm<float, true, false>(p, backward, s); }
+        else { if (ln) launch_norm<float, false, true>(p, backward, s); else launch_norm<float, false, false>(p, backward, s); }
+    } else {
+        if (vec) { if (ln) launch_norm<bf16_t, true, true>(p, backward, s); else launch_norm<bf16_t, true, false>(p, backward, s); }
+        else { if (ln) launch_norm<bf16_t, false, true>(p, backward, s); else launch_norm<bf16_t, false, false>(p, backward, s); }
+    }
+    XRL_CHECK_LAUNCH();
+    return XRL_OK;
+}
+
+}  // namespace xrl
+
+using namespace xrl;
+
+extern "C" int64_t xrl_block_norm_workspace_floats(const xrl_block_norm_t* p) {
+    if (!p || check_norm(*p)) return XRL_EINVAL;
+    return (int64_t)norm_lines(*p) * NORM_SUMS * p->D;
+}
+
+extern "C" int xrl_block_norm_forward(const xrl_block_norm_t* pp, xrl_stream_t stream) {
+    XRL_CHECK_ARG(pp != nullptr);
+    const xrl_block_norm_t& p = *pp;
+    if (int rc = check_norm(p)) return rc;
+    if (p.N == 0) return XRL_OK;
+    XRL_CHECK_ARG(p.x && p.u && p.y);
+    return run_norm(p, false, as_stream(stream));
+}
+
+extern "C" int xrl_block_norm_backward(const xrl_block_norm_t* pp, xrl_stream_t stream) {
+    XRL_CHECK_ARG(pp != nullptr);
+    const xrl_block_norm_t& p = *pp;
+    if (int rc = check_norm(p)) return rc;
+    XRL_CHECK_ARG(!p.d_gate || p.gate);
+    XRL_CHECK_ARG(p.N == 0 || (p.x && p.u && p.d_x && p.d_u && (p.d_y || p.d_n) && p.workspace));
+    XRL_CHECK_ARG(p.workspace_floats >= (int64_t)norm_lines(p) * NORM_SUMS * p.D);
+    if (p.N > 0)
+        if (int rc = run_norm(p, true, as_stream(stream))) return rc;
+    if (p.d_scale || p.d_w_post || p.d_b_post || p.d_w_pre || p.d_b_pre) {
+        hipLaunchKernelGGL(block_norm_sums_kernel, dim3((NORM_SUMS * p.D + 15) / 16), dim3(1024), 0, as_stream(stream), p, norm_lines(p));
+        XRL_CHECK_LAUNCH();
+    }
+    return XRL_OK;
+}
