@@ -1,10 +1,10 @@
-"""Subprocess vector env whose step data travels through shared, page-locked host memory.
+"""Subprocess vector env whose step data travels through shared host memory.
 
 The reference's SubprocVecEnv (xuance/environment/vector_envs/subprocess/subproc_vec_env.py:8-150) pickles every
 observation / reward / flag / info dict through a Pipe per worker per step, and the agent then copies the stacked arrays
 once more on their way to the device.  Here the workers write their slice of ONE shared block -- actions in; observation,
 post-reset observation, reward, terminated, truncated, episode step / score out -- and the pipes carry a one-byte command
-and a one-byte acknowledgement.  The block is registered with the HIP runtime (hipHostRegister), so ``step_to_device``
+and a one-byte acknowledgement.  ``step_to_device`` copies the block into page-locked memory and
 moves a whole vector step into HBM with a single asynchronous DMA; the device tensors it returns are what
 ``HipOnPolicyBuffer.store`` / ``xrl_soa_store_step`` consume.
 
@@ -91,7 +91,7 @@ class ShmSubprocVecEnv:
         self.lay, nbytes = _layout(n, self.obs_shape, self.obs_dtype, self.act_dim)
         self.block = torch.zeros(nbytes, dtype=torch.uint8).share_memory_()
         self.v = _views(self.block, self.lay, n, self.obs_shape, self.obs_dtype, self.act_dim)
-        # the worker processes are fork()ed BEFORE this object makes its first HIP call (hipHostRegister, the device
+        # the worker processes are fork()ed BEFORE this object makes its first HIP call (the page-locked copy, the device
         # mirror): a child forked from a process whose HIP runtime is already live inherits runtime state it must never
         # use.  (If the caller initialised HIP earlier, create the vector env first -- or the workers simply never touch it:
         # they only see NumPy views of the shared block.)
@@ -112,9 +112,10 @@ class ShmSubprocVecEnv:
         self._pinned = False
         self._dma_done = None                                       # event of the last step_to_device copy
         if torch.cuda.is_available() and str(device).startswith("cuda"):
-            # page-lock the shared block in place: H2D copies from it are true asynchronous DMAs
-            err = torch.cuda.cudart().cudaHostRegister(self.block.data_ptr(), nbytes, 0)
-            self._pinned = int(err) == 0
+            # a page-locked copy of the shared block: H2D copies from it are true asynchronous DMAs (page-locking the shared memory itself
+            # is refused on some hosts, and the refusal then surfaces in a later, unrelated call)
+            self._stage = torch.zeros(nbytes, dtype=torch.uint8, pin_memory=True)
+            self._pinned = self._stage.is_pinned()
             self.dev_block = torch.zeros(nbytes, dtype=torch.uint8, device=device)
             d = lambda name, dt, shape: self.dev_block[self.lay[name][0]:self.lay[name][0] + self.lay[name][1]].view(dt).view(shape)
             tdt = torch.uint8 if self.obs_dtype == np.uint8 else torch.float32
@@ -145,7 +146,7 @@ class ShmSubprocVecEnv:
 
     def step_async(self, actions):
         self._assert_not_closed()
-        if self._dma_done is not None:                              # the previous step_to_device copy still reads the block
+        if self._dma_done is not None:                              # the previous step_to_device copy still reads its page-locked copy
             self._dma_done.synchronize()
             self._dma_done = None
         self.v["actions"][...] = np.asarray(actions, np.float32).reshape(self.num_envs, self.act_dim)
@@ -185,7 +186,8 @@ class ShmSubprocVecEnv:
             actions = actions.detach().to("cpu", torch.float32).numpy()
         self.step_async(actions)
         self._wait()
-        self.dev_block.copy_(self.block, non_blocking=self._pinned)
+        self._stage.copy_(self.block)                              # step_async waited for the copy that read it last
+        self.dev_block.copy_(self._stage, non_blocking=self._pinned)
         if self._pinned:
             self._dma_done = torch.cuda.Event()
             self._dma_done.record()
@@ -200,8 +202,6 @@ class ShmSubprocVecEnv:
             r.send_bytes(b"c")
         for p in self.ps:
             p.join(timeout=5)
-        if self._pinned:
-            torch.cuda.cudart().cudaHostUnregister(self.block.data_ptr())
         self.closed = True
 
     def _assert_not_closed(self):

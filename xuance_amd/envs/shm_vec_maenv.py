@@ -1,4 +1,4 @@
-"""Multi-agent subprocess vector env over shared, page-locked host memory -- the multi-agent twin of shm_vec_env.py
+"""Multi-agent subprocess vector env over shared host memory -- the multi-agent twin of shm_vec_env.py
 (SURVEY.md section 8f.3).
 
 The reference's SubprocVecMultiAgentEnv (xuance/environment/vector_envs/subprocess/subproc_vec_maenv.py:8-170) pickles, per
@@ -6,7 +6,7 @@ worker and per step, a list of (obs dict, reward dict, terminated dict, truncate
 reset_*) through a Pipe.  Here every worker writes its envs' slice of ONE shared block of fixed-size arrays -- actions in;
 per-agent observations, global state, action-availability masks (each also in its post-reset form), rewards, terminated
 flags, agent masks, truncated, episode step / per-agent episode scores out -- and the pipes carry a one-byte command and a
-one-byte acknowledgement.  The block is registered with the HIP runtime, so ``step_to_device`` moves a whole vector step
+one-byte acknowledgement.  ``step_to_device`` copies the block into page-locked memory and moves a whole vector step
 into HBM with one asynchronous DMA, already in the [n_envs, n_agents, ...] arrays the device-side agents consume.
 
 Same surface and auto-reset contract as the reference class (and as DummyVecMultiAgentEnv): ``reset() -> (obs_list,
@@ -133,8 +133,8 @@ class ShmSubprocVecMultiAgentEnv:
             wr.close()
         self.device, self._pinned, self._dma_done = device, False, None
         if torch.cuda.is_available() and str(device).startswith("cuda"):
-            err = torch.cuda.cudart().cudaHostRegister(self.block.data_ptr(), nbytes, 0)     # page-lock in place
-            self._pinned = int(err) == 0
+            self._stage = torch.zeros(nbytes, dtype=torch.uint8, pin_memory=True)            # page-locked copy (see shm_vec_env.py)
+            self._pinned = self._stage.is_pinned()
             self.dev_block = torch.zeros(nbytes, dtype=torch.uint8, device=device)
             tdt = {_F32: torch.float32, _U8: torch.uint8, _I32: torch.int32}
             self.dev = {k: self.dev_block[o:o + nb].view(tdt[dt]).view(shape) for k, (o, nb, dt, shape) in self.lay.items()
@@ -178,7 +178,7 @@ class ShmSubprocVecMultiAgentEnv:
 
     def step_async(self, actions):
         self._assert_not_closed()
-        if self._dma_done is not None:                              # the previous step_to_device copy still reads the block
+        if self._dma_done is not None:                              # the previous step_to_device copy still reads its page-locked copy
             self._dma_done.synchronize()
             self._dma_done = None
         if isinstance(actions, (list, tuple)) and isinstance(actions[0], dict):
@@ -228,7 +228,8 @@ class ShmSubprocVecMultiAgentEnv:
             actions = actions.detach().to("cpu", torch.float32).numpy()
         self.step_async(actions)
         self._wait()
-        self.dev_block.copy_(self.block, non_blocking=self._pinned)
+        self._stage.copy_(self.block)                              # step_async waited for the copy that read it last
+        self.dev_block.copy_(self._stage, non_blocking=self._pinned)
         if self._pinned:
             self._dma_done = torch.cuda.Event()
             self._dma_done.record()
@@ -243,8 +244,6 @@ class ShmSubprocVecMultiAgentEnv:
             r.send_bytes(b"c")
         for p in self.ps:
             p.join(timeout=5)
-        if self._pinned:
-            torch.cuda.cudart().cudaHostUnregister(self.block.data_ptr())
         self.closed = True
 
     def _assert_not_closed(self):
