@@ -5,80 +5,46 @@
 // is the forward pass for (a, b, c) = (q, k, v) and the gradients for
 //     d_q: (d_out, v, k), S_in = state^T;     d_k: (v, d_out, q) and d_v: (k, q, d_out) in reversed time, S_in = d_state_out(^T), off = 0,
 // because S_t meets d S_t exactly where o_t meets q_t.  A launch runs one job (forward) or three (backward) of it.
-#include "io16.h"
+#include "linattn_mix.h"
 
 namespace xrl {
 
-struct mix_job_t {
-    const void* a; const void* b; const void* c; void* out;
-    int64_t sa[3], sb[3], sc[3], so[3];
-    int da, dc;
-    const float* s_in; float* s_out;      // [B][H][dk][dv], element (d, e) at d * sd + e * se
-    int sd, se;
-    int reverse, off;
-    float scale_p, scale_s, scale_b;      // of the products a.b, of a S, of b (x) c in the state
+// The segments of a split time axis joined: every segment's own state becomes the state before it, S_in carried on past the last one is s_out.
+struct scan_job_t {
+    float* states; const float* carry;            // [row and head][segment][kv], [row and head][segment][2]
+    const float* s_in; float* s_out;              // NULL or [B][H][.][.]
+    int dc, sd, se;
+    int stop_at_first;                            // s_out is 0 where the first step has a reset (reversed time)
 };
-struct mix_t {
-    mix_job_t job[3];
-    const float* log_decay; const int32_t* lengths; const float* reset;
-    int T, B, H, kv;
+struct scan_t {
+    scan_job_t job[2];
+    const float* reset; const int32_t* lengths;
+    int T, H, kv, n_seg;
 };
 
-// The recurrence, one token after another: a workgroup holds the state columns [64 z, 64 z + 64) of one row, head and job.
-template <typename E>
-__global__ void __launch_bounds__(256) linattn_mix_kernel(mix_t p) {
-    const mix_job_t& J = p.job[blockIdx.y];
-    const int bh = blockIdx.x, b = bh / p.H, h = bh % p.H;
-    const int col = threadIdx.x & 63, grp = threadIdx.x >> 6, e = blockIdx.z * 64 + col;
-    if ((int)blockIdx.z * 64 >= J.dc) return;
-    __shared__ float la[128], lb[128], part[4][64];
-    const int n = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
-    const float lam = expf(fminf(p.log_decay[h], 0.f));
-    const bool own = e < J.dc;
-    float s[32];
+__global__ void __launch_bounds__(256) linattn_scan_kernel(scan_t p) {
+    const scan_job_t& J = p.job[blockIdx.z];
+    const int bh = blockIdx.y, x = blockIdx.x * 256 + threadIdx.x;
+    if (x >= p.kv) return;
+    const int64_t at = (int64_t)bh * p.kv + (int64_t)(x / J.dc) * J.sd + (int64_t)(x % J.dc) * J.se;
+    float* s = J.states + (int64_t)bh * p.n_seg * p.kv + x;
+    const float* c = J.carry + (int64_t)bh * p.n_seg * 2;
+    float cur = J.s_in ? J.s_in[at] : 0.f;
+    for (int i = 0; i < p.n_seg; i += 8) {
+        float own[8];
 #pragma unroll
-    for (int m = 0; m < 32; ++m) {
-        const int d = grp + 4 * m;
-        s[m] = (J.s_in && own && d < J.da) ? J.s_in[(size_t)bh * p.kv + (size_t)d * J.sd + (size_t)e * J.se] : 0.f;
+        for (int q = 0; q < 8; ++q) own[q] = i + q < p.n_seg ? s[(int64_t)(i + q) * p.kv] : 0.f;
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+            if (i + q < p.n_seg) {
+                s[(int64_t)(i + q) * p.kv] = cur;
+                cur = __builtin_fmaf(cur, c[2 * (i + q)], cur * c[2 * (i + q) + 1]) + own[q];
+            }
     }
-    const E* pa = (const E*)J.a + b * J.sa[1] + h * J.sa[2];
-    const E* pb = (const E*)J.b + b * J.sb[1] + h * J.sb[2];
-    const E* pc = (const E*)J.c + b * J.sc[1] + h * J.sc[2];
-    E* po = (E*)J.out + b * J.so[1] + h * J.so[2];
-    // off = 1: S decays before every token; off = 0 (reversed time): S_in meets the first token as it is, and S leaves decayed
-    for (int i = 0; i < n; ++i) {
-        const int64_t t = J.reverse ? n - 1 - i : i;
-        __syncthreads();
-        if (threadIdx.x < 128) la[threadIdx.x] = threadIdx.x < J.da ? io_load(pa + t * J.sa[0] + threadIdx.x) : 0.f;
-        else lb[threadIdx.x - 128] = threadIdx.x - 128 < J.da ? io_load(pb + t * J.sb[0] + threadIdx.x - 128) : 0.f;
-        const float c = own ? io_load(pc + t * J.sc[0] + e) : 0.f;
-        // a reset before step t cuts t off from what came before; in reversed time from what came after: the reset of step t + 1
-        const int64_t rt = J.reverse ? t + 1 : t;
-        const bool cut = p.reset && rt < n && p.reset[rt * p.B + b] != 0.f;
-        const float keep = cut ? 0.f : (J.off == 1 || i > 0) ? lam : 1.f;
-        __syncthreads();
-        float acc_p = 0.f, acc_s = 0.f;
-#pragma unroll
-        for (int m = 0; m < 32; ++m) {
-            const int d = grp + 4 * m;
-            const float prev = cut ? 0.f : keep * s[m], now = lb[d] * c;
-            acc_s += la[d] * prev;
-            acc_p += la[d] * now;
-            s[m] = prev + J.scale_b * now;
-        }
-        part[grp][col] = J.scale_s * acc_s + J.scale_p * acc_p;
-        __syncthreads();
-        if (grp == 0 && own) io_store(po + t * J.so[0] + e, (part[0][col] + part[1][col]) + (part[2][col] + part[3][col]));
-    }
-    for (int64_t t = n; t < p.T; ++t)
-        if (grp == 0 && own) io_store(po + t * J.so[0] + e, 0.f);
-    if (J.s_out && own) {
-        const float last = (J.off == 0 && n > 0) ? ((p.reset && p.reset[b] != 0.f) ? 0.f : lam) : 1.f;
-#pragma unroll
-        for (int m = 0; m < 32; ++m) {
-            const int d = grp + 4 * m;
-            if (d < J.da) J.s_out[(size_t)bh * p.kv + (size_t)d * J.sd + (size_t)e * J.se] = last == 0.f ? 0.f : last * s[m];
-        }
+    if (J.s_out) {
+        const int b = bh / p.H;
+        const bool none = J.stop_at_first && p.reset && p.reset[b] != 0.f && p.T > 0 && (!p.lengths || p.lengths[b] > 0);
+        J.s_out[at] = none ? 0.f : cur;
     }
 }
 
@@ -129,7 +95,7 @@ __global__ void __launch_bounds__(256) linattn_step_kernel(xrl_linattn_t p) {
 
 static int check_sizes(const xrl_linattn_t& p) {
     XRL_CHECK_ARG(p.T >= 0 && p.B >= 0 && p.H >= 1 && p.dk >= 1 && p.dk <= 128 && p.dv >= 1 && p.dv <= 128);
-    XRL_CHECK_ARG((int64_t)p.B * p.H <= 0x7fffffff);
+    XRL_CHECK_ARG((int64_t)p.B * p.H <= 1 << 24);
     XRL_CHECK_ARG(p.dtype == XRL_F32 || p.dtype == XRL_BF16);
     return XRL_OK;
 }
@@ -163,14 +129,83 @@ static void backward_jobs(const xrl_linattn_t& p, mix_job_t* j) {
     v.reverse = 1; v.off = 0; v.scale_p = v.scale_b = p.scale; v.scale_s = 1.f;
 }
 
-static int run_jobs(const xrl_linattn_t& p, mix_t& m, int n_jobs, xrl_stream_t stream) {
+static bool rows16(const void* p, const int64_t* s, int d, int unit, int bytes) {
+    return d % unit == 0 && s[0] % unit == 0 && s[1] % unit == 0 && s[2] % unit == 0 && reinterpret_cast<uintptr_t>(p) % bytes == 0;
+}
+
+static void set_vec(mix_job_t& j, int dtype) {
+    const int unit = dtype == XRL_F32 ? 4 : 8;
+    j.vec = (rows16(j.a, j.sa, j.da, unit, 16) ? 1 : 0) | (rows16(j.b, j.sb, j.da, unit, 16) ? 2 : 0) | (rows16(j.c, j.sc, j.dc, unit, 16) ? 4 : 0) |
+            (rows16(j.out, j.so, j.dc, 4, dtype == XRL_F32 ? 16 : 8) ? 8 : 0);
+}
+
+// Segments of the time axis: where rows x heads x jobs are too few workgroups for the chip, the axis is cut so that about two per compute unit
+// run, four chunks each at least (a segment reads b and c twice: once for its state, once for its outputs).
+static int segments(const xrl_linattn_t& p, int n_jobs, int* seg_chunks) {
+    const int64_t wgs = (int64_t)p.B * p.H * n_jobs;
+    const int chunks = (p.T + CH - 1) / CH;
+    int n = 1;
+    if (wgs > 0 && wgs < 256) {
+        const int64_t want = (512 + wgs - 1) / wgs;
+        n = (int)(want < chunks / 4 ? want : chunks / 4);
+        if (n < 1) n = 1;
+    }
+    *seg_chunks = chunks > 0 ? (chunks + n - 1) / n : 1;
+    return chunks > 0 ? (chunks + *seg_chunks - 1) / *seg_chunks : 1;
+}
+
+static int64_t split_floats(const xrl_linattn_t& p, int n_seg, int n_states) {
+    return n_seg > 1 ? (int64_t)n_states * p.B * p.H * n_seg * (p.dk * p.dv + 2) : 0;
+}
+
+static int launch(const xrl_linattn_t& p, const mix_t& m, hipStream_t s) {
+    int da = 0, dc = 0;
+    for (int i = 0; i < m.n_jobs; ++i) { da = da > m.job[i].da ? da : m.job[i].da; dc = dc > m.job[i].dc ? dc : m.job[i].dc; }
+    return p.dtype == XRL_F32 ? launch_mix_f32(m, da, dc, s) : launch_mix_bf16(m, da, dc, s);
+}
+
+// jobs: the outputs to make; holder[i]: the job whose split states job i starts from, itself or one of the same state transposed
+static int run_jobs(const xrl_linattn_t& p, mix_t& m, int n_jobs, const int* holder, hipStream_t s) {
     m.log_decay = p.log_decay; m.lengths = p.lengths; m.reset = p.reset;
-    m.T = p.T; m.B = p.B; m.H = p.H; m.kv = p.dk * p.dv;
-    const dim3 grid(p.B * p.H, n_jobs, 2);
-    if (p.dtype == XRL_F32) hipLaunchKernelGGL(linattn_mix_kernel<float>, grid, dim3(256), 0, as_stream(stream), m);
-    else hipLaunchKernelGGL(linattn_mix_kernel<bf16_t>, grid, dim3(256), 0, as_stream(stream), m);
+    m.T = p.T; m.B = p.B; m.H = p.H; m.kv = p.dk * p.dv; m.n_jobs = n_jobs;
+    m.n_seg = segments(p, n_jobs, &m.seg_chunks);
+    for (int i = 0; i < n_jobs; ++i) { set_vec(m.job[i], p.dtype); m.job[i].s_row = m.kv; }
+    if (m.n_seg == 1) return launch(p, m, s);
+    mix_t st = m;
+    scan_t sc{};
+    sc.reset = p.reset; sc.lengths = p.lengths; sc.T = p.T; sc.H = p.H; sc.kv = m.kv; sc.n_seg = m.n_seg;
+    const int64_t bhs = (int64_t)p.B * p.H * m.n_seg;
+    int n = 0, slot[3] = {0, 0, 0};
+    for (int i = 0; i < n_jobs; ++i)
+        if (holder[i] == i) slot[i] = n++;
+    float* carries = p.workspace + n * bhs * m.kv;
+    for (int i = 0; i < n_jobs; ++i) {
+        if (holder[i] != i) continue;
+        const mix_job_t& j = m.job[i];
+        mix_job_t& t = st.job[slot[i]];
+        t = j;
+        t.s_in = nullptr;
+        t.s_out = p.workspace + slot[i] * bhs * m.kv;
+        t.carry = carries + slot[i] * bhs * 2;
+        scan_job_t& q = sc.job[slot[i]];
+        q.states = t.s_out; q.carry = t.carry; q.s_in = j.s_in; q.s_out = j.s_out; q.dc = j.dc; q.sd = j.sd; q.se = j.se; q.stop_at_first = j.off == 0;
+    }
+    st.n_jobs = n; st.states_only = 1;
+    if (int rc = launch(p, st, s)) return rc;
+    hipLaunchKernelGGL(linattn_scan_kernel, dim3((m.kv + 255) / 256, p.B * p.H, n), dim3(256), 0, s, sc);
     XRL_CHECK_LAUNCH();
-    return XRL_OK;
+    for (int i = 0; i < n_jobs; ++i) {
+        mix_job_t& j = m.job[i];
+        j.s_in = p.workspace + slot[holder[i]] * bhs * m.kv;
+        if (holder[i] == i) { j.sd = j.dc; j.se = 1; }
+        else { j.sd = 1; j.se = m.job[holder[i]].dc; }
+    }
+    return launch(p, m, s);
+}
+
+int init_linattn() {
+    if (int rc = init_mix_f32()) return rc;
+    return init_mix_bf16();
 }
 
 }  // namespace xrl
@@ -178,9 +213,9 @@ static int run_jobs(const xrl_linattn_t& p, mix_t& m, int n_jobs, xrl_stream_t s
 using namespace xrl;
 
 extern "C" int64_t xrl_linattn_workspace_floats(const xrl_linattn_t* p, int backward) {
-    (void)backward;
     if (!p || check_sizes(*p)) return XRL_EINVAL;
-    return 0;
+    int chunks;
+    return split_floats(*p, segments(*p, backward ? 3 : 1, &chunks), backward ? 2 : 1);
 }
 
 extern "C" int xrl_linattn_forward(const xrl_linattn_t* pp, xrl_stream_t stream) {
@@ -189,9 +224,12 @@ extern "C" int xrl_linattn_forward(const xrl_linattn_t* pp, xrl_stream_t stream)
     if (int rc = check_sizes(p)) return rc;
     XRL_CHECK_ARG(p.log_decay && (p.T == 0 || p.B == 0 || (p.q && p.k && p.v && p.out)));
     if (p.B == 0) return XRL_OK;
+    const int64_t need = xrl_linattn_workspace_floats(pp, 0);
+    XRL_CHECK_ARG(need == 0 || (p.workspace && p.workspace_floats >= need));
     mix_t m{};
     m.job[0] = forward_job(p);
-    return run_jobs(p, m, 1, stream);
+    const int holder[1] = {0};
+    return run_jobs(p, m, 1, holder, as_stream(stream));
 }
 
 extern "C" int xrl_linattn_backward(const xrl_linattn_t* pp, xrl_stream_t stream) {
@@ -201,9 +239,12 @@ extern "C" int xrl_linattn_backward(const xrl_linattn_t* pp, xrl_stream_t stream
     XRL_CHECK_ARG(p.log_decay && (p.T == 0 || p.B == 0 || (p.q && p.k && p.v && p.d_out && p.d_q && p.d_k && p.d_v)));
     XRL_CHECK_ARG(!p.d_state || p.d_state != p.d_state_out);         // d_k's job reads d_state_out while d_v's writes d_state
     if (p.B == 0) return XRL_OK;
+    const int64_t need = xrl_linattn_workspace_floats(pp, 1);
+    XRL_CHECK_ARG(need == 0 || (p.workspace && p.workspace_floats >= need));
     mix_t m{};
     backward_jobs(p, m.job);
-    return run_jobs(p, m, 3, stream);
+    const int holder[3] = {0, 2, 2};                                 // d_k starts from the same states as d_v, transposed
+    return run_jobs(p, m, 3, holder, as_stream(stream));
 }
 
 extern "C" int xrl_linattn_step(const xrl_linattn_t* pp, xrl_stream_t stream) {

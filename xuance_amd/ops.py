@@ -1302,6 +1302,7 @@ def _workspace(given, floats, device):
 
 
 def _linattn(q, k, v, log_decay, scale, lengths, reset, state, state_out):
+    init_device()
     p = LinAttn()
     _need(q.dim() == 4 and v.dim() == 4, f"q, k, v: [T, B, H, d] each, got {tuple(q.shape)}, {tuple(v.shape)}")
     dev = torch.cuda.current_device()
