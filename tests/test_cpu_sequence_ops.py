@@ -1,5 +1,4 @@
-"""Host side of the sequence-policy operators: struct layouts, what the C entry points and the Python wrappers refuse (nothing is launched), and the
-test of shared memory between a call's tensors."""
+"""Host side of the sequence-policy operators: struct layouts, and what the C entry points and the Python wrappers refuse (nothing is launched)."""
 import ctypes
 import math
 import os
@@ -12,7 +11,8 @@ from conftest import ROOT
 
 
 def test_structs_match_the_header(tmp_path):
-    from xuance_amd import _lib
+    from xuance_amd import _lib, ops
+    assert [f.size for f in (ops._LINATTN, ops._BLOCK_NORM, ops._DISTILL)] == [ctypes.sizeof(c) for c in (_lib.LinAttn, _lib.BlockNorm, _lib.Distill)]
     pairs = {"xrl_linattn_t": _lib.LinAttn, "xrl_block_norm_t": _lib.BlockNorm, "xrl_distill_t": _lib.Distill}
     src = '#include "xrl_hip.h"\n#include <stdio.h>\n#include <stddef.h>\nint main(){\n'
     for cname, cls in pairs.items():
@@ -60,7 +60,6 @@ def test_linattn_refuses(entry, bad):
 
 def test_linattn_refuses_more():
     assert call("xrl_linattn_forward", None) < 0
-    assert call("xrl_linattn_backward", lin(d_state=4096)) < 0                 # d_state in place of d_state_out
     assert call("xrl_linattn_step", lin(T=2)) < 0
     assert call("xrl_linattn_step", lin(T=1, state=None)) < 0
     assert call("xrl_linattn_backward", lin(d_k=None)) < 0
@@ -102,13 +101,24 @@ def test_distill_refuses(bad):
 # --------------------------------------------------------------------------------------------------- the wrappers' own checks
 @pytest.fixture
 def host_ops(monkeypatch):
-    """The wrappers with host tensors let through and the launches counted instead of made."""
-    from xuance_amd import ops
+    """The wrappers with host tensors let through: the C entry points look at them and, without a device, fail to launch; that counts as let through."""
+    from xuance_amd import _lib, ops
+    if torch.cuda.is_available():
+        pytest.skip("host tensors would reach a kernel")
     made = []
+
+    def call(name, *a):
+        rc = getattr(_lib.load(), name)(*a)
+        if rc == -2:                                                            # XRL_EHIP
+            made.append(name)
+        elif rc != 0:
+            raise ops.XrlError(_lib.load().xrl_last_error().decode())
     monkeypatch.setattr(ops, "_on_device", lambda t, device: True)
-    monkeypatch.setattr(ops, "call", lambda name, *a: made.append(name))
+    monkeypatch.setattr(ops, "call", call)
+    monkeypatch.setattr(ops, "init_device", lambda: None)
     monkeypatch.setattr(ops, "stream_ptr", lambda: None)
     monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
     ops.made = made
     yield ops
     del ops.made
@@ -116,7 +126,7 @@ def host_ops(monkeypatch):
 
 def test_wrappers_refuse_wrong_tensors(host_ops):
     ops = host_ops
-    t = torch.zeros
+    t = torch.zeros                                                             # every call its own, unless it says otherwise
     good = dict(q=t(5, 2, 3, 8), k=t(5, 2, 3, 8), v=t(5, 2, 3, 4), out=t(5, 2, 3, 4), log_decay=t(3))
     ops.linattn_forward(**good, lengths=t(2).int(), reset=t(5, 2), state=t(2, 3, 8, 4), state_out=t(2, 3, 8, 4))
     assert ops.made == ["xrl_linattn_forward"]
@@ -128,6 +138,7 @@ def test_wrappers_refuse_wrong_tensors(host_ops):
         with pytest.raises(ops.XrlError):
             ops.linattn_forward(**{**good, **bad})
     s = t(2, 3, 8, 4)
+    ops.linattn_backward(good["q"], good["k"], good["v"], good["out"], t(5, 2, 3, 8), t(5, 2, 3, 8), t(5, 2, 3, 4), good["log_decay"], d_state_out=s)
     with pytest.raises(ops.XrlError):                                           # the gradient in place of the gradient it is made from
         ops.linattn_backward(good["q"], good["k"], good["v"], good["out"], t(5, 2, 3, 8), t(5, 2, 3, 8), t(5, 2, 3, 4), good["log_decay"], d_state_out=s, d_state=s)
     d = t(5, 2, 3, 8)
@@ -159,21 +170,50 @@ def test_wrappers_refuse_wrong_tensors(host_ops):
             ops.distill_loss(**{**c, **bad})
 
 
-def test_shared_memory_between_tensors():
-    from xuance_amd import ops
-    rows = torch.zeros(5, 2, 3 * 12)
+def test_outputs_share_no_memory(host_ops):
+    """Slices of one buffer are outputs beside each other; anything that overlaps is refused, and so are outputs whose own elements do."""
+    ops = host_ops
+    rows, ld = torch.zeros(5, 2, 3 * 12), torch.zeros(3)
     part = [rows[..., 12 * i:12 * i + 12].view(5, 2, 3, 4) for i in range(3)]
-    ops._apart({"a": part[0], "b": part[1], "c": part[2]}, {"d": torch.zeros(5, 2, 3, 4)})
-    ops._apart({"a": rows[:, 0]}, {"b": rows[:, 1]})
-    ops._apart({"a": rows[:2]}, {"b": rows[2:]})
-    for a, b in ((part[0], part[0]), (rows[:3], rows[2:]), (rows[..., :13], rows[..., 12:]), (rows, part[1]), (rows.view(-1), rows[0])):
+    far = [torch.zeros(5, 2, 3, 4) for _ in range(4)]
+    back = lambda dq, dk, dv, q=far[0]: ops.linattn_backward(q, far[1], far[2], far[3], dq, dk, dv, ld)      # noqa: E731
+    back(*part)
+    back(torch.zeros(2, 5, 3, 4).transpose(0, 1), torch.zeros(3, 5, 2, 4).permute(1, 2, 0, 3), torch.zeros(5, 2, 3, 6)[..., 1:5])
+    both = torch.zeros(10, 2, 3, 4)
+    back(both[:5], both[5:], part[0])
+    back(both[::2], both[1::2], part[0])
+    assert ops.made == ["xrl_linattn_backward"] * 4
+    wide = torch.zeros(5, 2, 3, 7)
+    for bad in ((part[0], part[0], part[1]), (both[:5], both[4:9], part[0]), (wide[..., :4], wide[..., 3:], part[0]), (part[0], part[1], far[1]),
+                (torch.zeros(1, 2, 3, 4).expand(5, -1, -1, -1), part[0], part[1]), (torch.zeros(400).as_strided((5, 2, 3, 4), (24, 12, 2, 1)), part[0], part[1]),
+                (torch.zeros(400).as_strided((5, 2, 3, 4), (20, 12, 4, 1)), part[0], part[1])):
+        with pytest.raises(ops.XrlError, match="share memory"):
+            back(*bad)
+    x = torch.zeros(6, 8)
+    y = torch.zeros(6, 16)
+    ops.block_norm_forward(x, y[:, :8], x, y[:, 8:])
+    with pytest.raises(ops.XrlError, match="share memory"):
+        ops.block_norm_forward(x, y[:, :8], y[:, :8])
+    with pytest.raises(ops.XrlError, match="share memory"):
+        ops.block_norm_forward(y[:, :8], x, y[:, 1:9])
+    w = torch.zeros(8)
+    with pytest.raises(ops.XrlError, match="share memory"):
+        ops.block_norm_backward(x, torch.zeros(6, 8), torch.zeros(6, 8), None, torch.zeros(6, 8), torch.zeros(6, 8), d_scale=w, d_w_post=w, workspace=torch.zeros(4096))
+    ws = torch.zeros(4096)
+    with pytest.raises(ops.XrlError, match="share memory"):
+        ops.block_norm_backward(x, torch.zeros(6, 8), torch.zeros(6, 8), None, torch.zeros(6, 8), ws[:48].view(6, 8), workspace=ws)
+
+
+def test_a_captured_call_brings_its_workspace(host_ops):
+    ops = host_ops
+    need = ops.linattn_workspace_floats(30000, 1, 1, 4, 4)
+    assert need > 0
+    t = lambda: torch.zeros(30000, 1, 1, 4)                                     # noqa: E731
+    a = (t(), t(), t(), t(), torch.zeros(1))
+    for ws in (None, torch.zeros(need - 1), torch.zeros(need).double(), torch.zeros(2 * need)[::2], torch.zeros(need + 1)[1:]):
         with pytest.raises(ops.XrlError):
-            ops._apart({"a": a}, {"b": b})
-    ops._apart({"a": part[0]}, {"b": part[0]}, {("a", "b")})
+            ops.linattn_forward(*a, workspace=ws)
+    ops.linattn_forward(*a, workspace=torch.zeros(need))
+    assert ops.made == ["xrl_linattn_forward"]
     with pytest.raises(ops.XrlError):
-        ops._apart({"a": part[0]}, {"b": part[0].transpose(0, 0)[1:]}, {("a", "b")})
-    for bad in (torch.zeros(1, 4).expand(3, 4), torch.zeros(10).as_strided((4, 4), (2, 1))):
-        with pytest.raises(ops.XrlError):
-            ops._output("a", bad)
-    for good in (torch.zeros(4, 6).t(), torch.zeros(4, 6)[:, 1:3], torch.zeros(0, 3), torch.zeros(3, 1, 4).expand(3, 1, 4)):
-        ops._output("a", good)
+        ops.block_norm_backward(torch.zeros(6, 8), torch.zeros(6, 8), torch.zeros(6, 8), None, torch.zeros(6, 8), torch.zeros(6, 8))

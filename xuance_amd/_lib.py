@@ -414,12 +414,12 @@ class Distill(C.Structure):
 
 
 _SIGS = {
-    "xrl_linattn_forward": [C.POINTER(LinAttn), c_void_p],
-    "xrl_linattn_backward": [C.POINTER(LinAttn), c_void_p],
-    "xrl_linattn_step": [C.POINTER(LinAttn), c_void_p],
-    "xrl_block_norm_forward": [C.POINTER(BlockNorm), c_void_p],
-    "xrl_block_norm_backward": [C.POINTER(BlockNorm), c_void_p],
-    "xrl_distill_loss": [C.POINTER(Distill), c_void_p],
+    "xrl_linattn_forward": [c_void_p, c_void_p],
+    "xrl_linattn_backward": [c_void_p, c_void_p],
+    "xrl_linattn_step": [c_void_p, c_void_p],
+    "xrl_block_norm_forward": [c_void_p, c_void_p],
+    "xrl_block_norm_backward": [c_void_p, c_void_p],
+    "xrl_distill_loss": [c_void_p, c_void_p],
     "xrl_marl_select_actions": [C.POINTER(MarlAct), c_void_p],
     "xrl_ppo_fused_minibatch": [C.POINTER(PpoFused), c_void_p],
     "xrl_ppo_trunk_chained": [C.POINTER(PpoFused), C.POINTER(OptChain), c_void_p],
@@ -582,9 +582,9 @@ def load():
     lib.xrl_rollout_wide_words.restype = c_int
     lib.xrl_rollout_wide_words.argtypes = []
     lib.xrl_linattn_workspace_floats.restype = c_int64
-    lib.xrl_linattn_workspace_floats.argtypes = [C.POINTER(LinAttn), c_int]
+    lib.xrl_linattn_workspace_floats.argtypes = [c_void_p, c_int]
     lib.xrl_block_norm_workspace_floats.restype = c_int64
-    lib.xrl_block_norm_workspace_floats.argtypes = [C.POINTER(BlockNorm)]
+    lib.xrl_block_norm_workspace_floats.argtypes = [c_void_p]
     for name, args in _SIGS.items():
         fn = getattr(lib, name)
         fn.argtypes = args
@@ -609,4 +609,4 @@ def ptr(t):
 
 def stream_ptr():
     import torch
-    return torch.cuda.current_stream().cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())       # current_stream() builds a Stream object around it

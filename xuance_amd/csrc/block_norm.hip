@@ -6,6 +6,7 @@
 // pass recomputes p, y and both statistics from the x, u and gate it needs anyway.  A row lives in the registers of L lanes, 8 values
 // each, from its one load to its one store; the parameters and the gradient sums over the rows stay in registers over all rows of a
 // workgroup.  Those sums leave as one line of partials per workgroup and a second launch adds the lines in a fixed order (no atomics).
+#include "args.h"
 #include "io16.h"
 
 namespace xrl {
@@ -20,64 +21,44 @@ struct norm_geom {
     static constexpr int WAVES = THREADS / 64;
 };
 
-// lane's m-th value of a row: 8 neighbours where the rows allow 16-byte accesses, else one every L
-template <int L, bool VEC>
-__device__ __forceinline__ int norm_at(int lane, int m) { return VEC ? lane * NV + m : lane + L * m; }
-
-template <typename E, int L, bool VEC>
-__device__ __forceinline__ void norm_load(const E* row, int lane, int D, float (&v)[NV]) {
-    if (VEC) {
+// eight neighbouring values of a row as they are stored; absent ones 0
+template <typename E>
+struct row8 {
+    static constexpr int PER = row16<E>::PER, N = NV / PER;
+    u32x4_t v[N];
+    __device__ __forceinline__ void load(const E* row, int at, int D) {
+        typedef row16<E> R;
 #pragma unroll
-        for (int m = 0; m < NV; ++m) v[m] = 0.f;
-        if (lane * NV < D) {
-            if (sizeof(E) == 4) {
+        for (int q = 0; q < N; ++q) { const u32x4_t zero = {0, 0, 0, 0}; v[q] = zero; }
+        if (at + NV <= D) {
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    const f32x4_t x = reinterpret_cast<const f32x4_t*>(row)[lane * 2 + q];
+            for (int q = 0; q < N; ++q) v[q] = R::load(row + at + PER * q);
+        } else if (at < D) {
 #pragma unroll
-                    for (int m = 0; m < 4; ++m) v[4 * q + m] = x[m];
-                }
-            } else {
-                const u32x4_t x = reinterpret_cast<const u32x4_t*>(row)[lane];
-#pragma unroll
-                for (int m = 0; m < 4; ++m) { v[2 * m] = __uint_as_float(x[m] << 16); v[2 * m + 1] = __uint_as_float(x[m] & 0xffff0000u); }
-            }
+            for (int m = 0; m < NV; ++m)
+                if (at + m < D) R::put(v[m / PER], m % PER, R::bits(row + at + m));
         }
-    } else {
-#pragma unroll
-        for (int m = 0; m < NV; ++m) v[m] = lane + L * m < D ? io_load(row + lane + L * m) : 0.f;
     }
-}
-
-template <typename E, int L, bool VEC>
-__device__ __forceinline__ void norm_store(E* row, int lane, int D, const float (&v)[NV]) {
-    if (VEC) {
-        if (lane * NV < D) {
-            if (sizeof(E) == 4) {
+    __device__ __forceinline__ void get(float (&f)[NV]) const {
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    const f32x4_t x = {v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
-                    reinterpret_cast<f32x4_t*>(row)[lane * 2 + q] = x;
-                }
-            } else {
-                const u32x4_t x = {cvt_pk_bf16(v[0], v[1]), cvt_pk_bf16(v[2], v[3]), cvt_pk_bf16(v[4], v[5]), cvt_pk_bf16(v[6], v[7])};
-                reinterpret_cast<u32x4_t*>(row)[lane] = x;
-            }
+        for (int m = 0; m < NV; ++m) f[m] = row16<E>::get(v[m / PER], m % PER);
+    }
+    static __device__ __forceinline__ void store(E* row, int at, int D, const float (&f)[NV]) {
+        typedef row16<E> R;
+        if (at + NV <= D) {
+#pragma unroll
+            for (int q = 0; q < N; ++q) R::store(row + at + PER * q, R::pack(f + PER * q));
+        } else if (at < D) {
+#pragma unroll
+            for (int m = 0; m < NV; ++m)
+                if (at + m < D) io_store(row + at + m, f[m]);
         }
-    } else {
-#pragma unroll
-        for (int m = 0; m < NV; ++m)
-            if (lane + L * m < D) io_store(row + lane + L * m, v[m]);
     }
-}
+};
 
-template <int L, bool VEC>
-__device__ __forceinline__ void norm_param(const float* p, int lane, int D, float missing, float (&v)[NV]) {
+__device__ __forceinline__ void norm_param(const float* p, int at, int D, float missing, float (&v)[NV]) {
 #pragma unroll
-    for (int m = 0; m < NV; ++m) {
-        const int e = norm_at<L, VEC>(lane, m);
-        v[m] = e < D ? (p ? p[e] : missing) : 0.f;
-    }
+    for (int m = 0; m < NV; ++m) v[m] = at + m < D ? (p ? p[at + m] : missing) : 0.f;
 }
 
 // Sums over the L lanes of a row.  Across waves through LDS with one barrier: consecutive sums use other slots of `scratch`, and a slot
@@ -117,15 +98,15 @@ struct row_sum_t {
 };
 
 // v := (v - mean) r (layer) or v r; returns r.  The variance is taken of the centred values (no difference of large sums).
-template <int L, bool VEC, bool LN>
-__device__ __forceinline__ float normalize(float (&v)[NV], int lane, int D, float inv_d, float eps, row_sum_t<L>& sum) {
+template <int L, bool LN>
+__device__ __forceinline__ float normalize(float (&v)[NV], int at, int D, float inv_d, float eps, row_sum_t<L>& sum) {
     if (LN) {
         float s = 0.f;
 #pragma unroll
         for (int m = 0; m < NV; ++m) s += v[m];
         const float mean = sum(s) * inv_d;
 #pragma unroll
-        for (int m = 0; m < NV; ++m) v[m] = norm_at<L, VEC>(lane, m) < D ? v[m] - mean : 0.f;
+        for (int m = 0; m < NV; ++m) v[m] = at + m < D ? v[m] - mean : 0.f;
     }
     float q = 0.f;
 #pragma unroll
@@ -136,30 +117,32 @@ __device__ __forceinline__ float normalize(float (&v)[NV], int lane, int D, floa
     return r;
 }
 
-template <typename E, int L, bool VEC, bool LN>
+template <typename E, int L, bool LN>
 __global__ void __launch_bounds__(norm_geom<L>::THREADS) block_norm_fwd_kernel(xrl_block_norm_t p) {
     using G = norm_geom<L>;
     __shared__ float2 scratch[3][16];
     row_sum_t<L> sum{scratch, 0};
-    const int lane = threadIdx.x % L, D = p.D;
+    const int lane = threadIdx.x % L, at = lane * NV, D = p.D;
     const float inv_d = 1.f / (float)D;
     float sc[NV], w0[NV], b0[NV], w1[NV], b1[NV];
-    norm_param<L, VEC>(p.scale, lane, D, 1.f, sc);
-    norm_param<L, VEC>(p.w_post, lane, D, 1.f, w0);
-    norm_param<L, VEC>(p.b_post, lane, D, 0.f, b0);
-    norm_param<L, VEC>(p.w_pre, lane, D, 1.f, w1);
-    norm_param<L, VEC>(p.b_pre, lane, D, 0.f, b1);
+    norm_param(p.scale, at, D, 1.f, sc);
+    norm_param(p.w_post, at, D, 1.f, w0);
+    norm_param(p.b_post, at, D, 0.f, b0);
+    norm_param(p.w_pre, at, D, 1.f, w1);
+    norm_param(p.b_pre, at, D, 0.f, b1);
     const int64_t step = (int64_t)gridDim.x * G::ROWS;
     for (int64_t base = (int64_t)blockIdx.x * G::ROWS; base < p.N; base += step) {       // whole workgroups go round: barriers inside
         const int64_t row = base + threadIdx.x / L;
         const bool live = row < p.N;
-        float x[NV] = {}, u[NV] = {}, g[NV] = {};
-        if (live) {
-            norm_load<E, L, VEC>((const E*)p.u + row * p.ld_u, lane, D, u);
-            norm_load<E, L, VEC>((const E*)p.x + row * p.ld_x, lane, D, x);
-            if (p.gate) norm_load<E, L, VEC>((const E*)p.gate + row * p.ld_gate, lane, D, g);
-        }
-        normalize<L, VEC, LN>(u, lane, D, inv_d, p.eps, sum);
+        const int width = live ? D : 0;
+        row8<E> rx, ru, rg;
+        ru.load((const E*)p.u + row * p.ld_u, at, width);
+        rx.load((const E*)p.x + row * p.ld_x, at, width);
+        if (p.gate) rg.load((const E*)p.gate + row * p.ld_gate, at, width);
+        float x[NV], u[NV], g[NV] = {};
+        ru.get(u); rx.get(x);
+        if (p.gate) rg.get(g);
+        normalize<L, LN>(u, at, D, inv_d, p.eps, sum);
         if (p.gate) {
             XRL_ACT_DISPATCH(p.gate_act, _Pragma("unroll") for (int m = 0; m < NV; ++m) g[m] = act_apply_c<ACT>(g[m]);)
         }
@@ -168,19 +151,19 @@ __global__ void __launch_bounds__(norm_geom<L>::THREADS) block_norm_fwd_kernel(x
             const float b = sc[m] * (u[m] * w0[m] + b0[m]);
             x[m] += p.gate ? g[m] * b : b;
         }
-        if (live) norm_store<E, L, VEC>((E*)p.y + row * p.ld_y, lane, D, x);
+        if (live) row8<E>::store((E*)p.y + row * p.ld_y, at, D, x);
         if (p.n) {
-            normalize<L, VEC, LN>(x, lane, D, inv_d, p.eps, sum);
+            normalize<L, LN>(x, at, D, inv_d, p.eps, sum);
 #pragma unroll
             for (int m = 0; m < NV; ++m) x[m] = x[m] * w1[m] + b1[m];
-            if (live) norm_store<E, L, VEC>((E*)p.n + row * p.ld_n, lane, D, x);
+            if (live) row8<E>::store((E*)p.n + row * p.ld_n, at, D, x);
         }
     }
 }
 
 // d := r (d - xhat mean(d xhat) [- mean(d)]): gradient through the normalisation
-template <int L, bool VEC, bool LN>
-__device__ __forceinline__ void normalize_back(float (&d)[NV], const float (&xhat)[NV], float r, int lane, int D, float inv_d,
+template <int L, bool LN>
+__device__ __forceinline__ void normalize_back(float (&d)[NV], const float (&xhat)[NV], float r, int at, int D, float inv_d,
                                                row_sum_t<L>& sum) {
     float a = 0.f, b = 0.f;
 #pragma unroll
@@ -188,35 +171,46 @@ __device__ __forceinline__ void normalize_back(float (&d)[NV], const float (&xha
     if (LN) { const float2 t = sum(a, b); a = t.x * inv_d; b = t.y * inv_d; }
     else a = sum(a) * inv_d;
 #pragma unroll
-    for (int m = 0; m < NV; ++m) d[m] = norm_at<L, VEC>(lane, m) < D ? r * (d[m] - xhat[m] * a - b) : 0.f;
+    for (int m = 0; m < NV; ++m) d[m] = at + m < D ? r * (d[m] - xhat[m] * a - b) : 0.f;
 }
 
-template <typename E, int L, bool VEC, bool LN>
+template <typename E, int L, bool LN>
 __global__ void __launch_bounds__(norm_geom<L>::THREADS) block_norm_bwd_kernel(xrl_block_norm_t p) {
     using G = norm_geom<L>;
     __shared__ float2 scratch[3][16];
     row_sum_t<L> sum{scratch, 0};
-    const int lane = threadIdx.x % L, D = p.D;
+    const int lane = threadIdx.x % L, at = lane * NV, D = p.D;
     const float inv_d = 1.f / (float)D;
     float sc[NV], w0[NV], b0[NV], w1[NV];
-    norm_param<L, VEC>(p.scale, lane, D, 1.f, sc);
-    norm_param<L, VEC>(p.w_post, lane, D, 1.f, w0);
-    norm_param<L, VEC>(p.b_post, lane, D, 0.f, b0);
-    norm_param<L, VEC>(p.w_pre, lane, D, 1.f, w1);
+    norm_param(p.scale, at, D, 1.f, sc);
+    norm_param(p.w_post, at, D, 1.f, w0);
+    norm_param(p.b_post, at, D, 0.f, b0);
+    norm_param(p.w_pre, at, D, 1.f, w1);
     float acc[NORM_SUMS][NV] = {};
+    // the next row is on its way while this one is worked on; 1024 threads leave no registers for that
+    constexpr bool AHEAD = L < 1024;
+    row8<E> rx, ru_, rg, ry_, rn;
+    auto request = [&](int64_t row) {
+        const int width = row < p.N ? D : 0;
+        ru_.load((const E*)p.u + row * p.ld_u, at, width);
+        rx.load((const E*)p.x + row * p.ld_x, at, width);
+        if (p.gate) rg.load((const E*)p.gate + row * p.ld_gate, at, width);
+        if (p.d_y) ry_.load((const E*)p.d_y + row * p.ld_d_y, at, width);
+        if (p.d_n) rn.load((const E*)p.d_n + row * p.ld_d_n, at, width);
+    };
+    if (AHEAD) request((int64_t)blockIdx.x * G::ROWS + threadIdx.x / L);
     const int64_t step = (int64_t)gridDim.x * G::ROWS;
     for (int64_t base = (int64_t)blockIdx.x * G::ROWS; base < p.N; base += step) {
         const int64_t row = base + threadIdx.x / L;
         const bool live = row < p.N;
-        float x[NV] = {}, u[NV] = {}, g[NV] = {}, dy[NV] = {}, dn[NV] = {}, t[NV];
-        if (live) {
-            norm_load<E, L, VEC>((const E*)p.u + row * p.ld_u, lane, D, u);
-            norm_load<E, L, VEC>((const E*)p.x + row * p.ld_x, lane, D, x);
-            if (p.gate) norm_load<E, L, VEC>((const E*)p.gate + row * p.ld_gate, lane, D, g);
-            if (p.d_y) norm_load<E, L, VEC>((const E*)p.d_y + row * p.ld_d_y, lane, D, dy);
-            if (p.d_n) norm_load<E, L, VEC>((const E*)p.d_n + row * p.ld_d_n, lane, D, dn);
-        }
-        const float ru = normalize<L, VEC, LN>(u, lane, D, inv_d, p.eps, sum);
+        float x[NV], u[NV], g[NV] = {}, dy[NV] = {}, dn[NV] = {}, t[NV];
+        if (!AHEAD) request(row);
+        ru_.get(u); rx.get(x);
+        if (p.gate) rg.get(g);
+        if (p.d_y) ry_.get(dy);
+        if (p.d_n) rn.get(dn);
+        if (AHEAD && base + step < p.N) request(row + step);
+        const float ru = normalize<L, LN>(u, at, D, inv_d, p.eps, sum);
         if (p.gate) {
             XRL_ACT_DISPATCH(p.gate_act, _Pragma("unroll") for (int m = 0; m < NV; ++m) g[m] = act_apply_c<ACT>(g[m]);)
         }
@@ -226,14 +220,14 @@ __global__ void __launch_bounds__(norm_geom<L>::THREADS) block_norm_bwd_kernel(x
                 const float b = sc[m] * (u[m] * w0[m] + b0[m]);
                 x[m] += p.gate ? g[m] * b : b;
             }
-            const float ry = normalize<L, VEC, LN>(x, lane, D, inv_d, p.eps, sum);
+            const float ry = normalize<L, LN>(x, at, D, inv_d, p.eps, sum);
 #pragma unroll
             for (int m = 0; m < NV; ++m) { acc[3][m] += dn[m] * x[m]; acc[4][m] += dn[m]; t[m] = dn[m] * w1[m]; }
-            normalize_back<L, VEC, LN>(t, x, ry, lane, D, inv_d, sum);
+            normalize_back<L, LN>(t, x, ry, at, D, inv_d, sum);
 #pragma unroll
             for (int m = 0; m < NV; ++m) dy[m] += t[m];
         }
-        if (live) norm_store<E, L, VEC>((E*)p.d_x + row * p.ld_d_x, lane, D, dy);
+        if (live) row8<E>::store((E*)p.d_x + row * p.ld_d_x, at, D, dy);
         // y = x + scale a p: with a the activated gate
 #pragma unroll
         for (int m = 0; m < NV; ++m) {
@@ -244,10 +238,10 @@ __global__ void __launch_bounds__(norm_geom<L>::THREADS) block_norm_bwd_kernel(x
         }
         if (p.d_gate) {
             XRL_ACT_DISPATCH(p.gate_act, _Pragma("unroll") for (int m = 0; m < NV; ++m) g[m] = dy[m] * act_grad_c<ACT>(g[m]);)
-            if (live) norm_store<E, L, VEC>((E*)p.d_gate + row * p.ld_d_gate, lane, D, g);
+            if (live) row8<E>::store((E*)p.d_gate + row * p.ld_d_gate, at, D, g);
         }
-        normalize_back<L, VEC, LN>(t, u, ru, lane, D, inv_d, sum);
-        if (live) norm_store<E, L, VEC>((E*)p.d_u + row * p.ld_d_u, lane, D, t);
+        normalize_back<L, LN>(t, u, ru, at, D, inv_d, sum);
+        if (live) row8<E>::store((E*)p.d_u + row * p.ld_d_u, at, D, t);
     }
     // partial sums: over the rows of a wave, then over the waves (in wave order), one line per workgroup
     float* line = p.workspace + (size_t)blockIdx.x * NORM_SUMS * D;
@@ -263,14 +257,13 @@ __global__ void __launch_bounds__(norm_geom<L>::THREADS) block_norm_bwd_kernel(x
         if (L > 64) {
 #pragma unroll
             for (int m = 0; m < NV; ++m) {
-                const int e = norm_at<L, VEC>(lane, m);
-                if (e < D) line[s * D + e] = acc[s][m];
+                if (at + m < D) line[s * D + at + m] = acc[s][m];
             }
         } else {
             __syncthreads();
             if ((int)(threadIdx.x & 63) < L) {
 #pragma unroll
-                for (int m = 0; m < NV; ++m) part[threadIdx.x >> 6][norm_at<L, VEC>(lane, m)] = acc[s][m];
+                for (int m = 0; m < NV; ++m) part[threadIdx.x >> 6][at + m] = acc[s][m];
             }
             __syncthreads();
             for (int e = threadIdx.x; e < D; e += G::THREADS) {
@@ -323,28 +316,37 @@ static int check_norm(const xrl_block_norm_t& p) {
     return XRL_OK;
 }
 
-static bool norm_vec(const xrl_block_norm_t& p, bool backward) {
-    const void* ptr[10] = {p.x, p.u, p.gate, p.y, p.n, p.d_y, p.d_n, p.d_x, p.d_u, p.d_gate};
-    const int64_t ld[10] = {p.ld_x, p.ld_u, p.ld_gate, p.ld_y, p.ld_n, p.ld_d_y, p.ld_d_n, p.ld_d_x, p.ld_d_u, p.ld_d_gate};
-    if (p.D % NV) return false;
-    const int unit = p.dtype == XRL_F32 ? 4 : 8;
-    for (int i = 0; i < 10; ++i) {
-        if (!ptr[i] || (backward ? (i == 3 || i == 4) : i > 4)) continue;
-        if ((reinterpret_cast<uintptr_t>(ptr[i]) & 15) || ld[i] % unit) return false;
+static int check_norm_tensors(const xrl_block_norm_t& p, bool backward) {
+    const int e = p.dtype == XRL_F32 ? 4 : 2;
+    auto rows = [&](const char* name, const void* ptr, int64_t ld, bool out) { return arg_t{name, ptr, e, 2, {p.N, p.D}, {ld, 1}, out}; };
+    auto vec = [&](const char* name, const void* ptr, bool out) { return arg_t{name, ptr, 4, 1, {p.D}, {1}, out}; };
+    const arg_t x = rows("x", p.x, p.ld_x, false), u = rows("u", p.u, p.ld_u, false), g = rows("gate", p.gate, p.ld_gate, false),
+                sc = vec("scale", p.scale, false), w0 = vec("w_post", p.w_post, false), b0 = vec("b_post", p.b_post, false),
+                w1 = vec("w_pre", p.w_pre, false), b1 = vec("b_pre", p.b_pre, false);
+    if (!backward) {
+        const arg_t a[] = {rows("y", p.y, p.ld_y, true), rows("n", p.n, p.ld_n, true), x, u, g, sc, w0, b0, w1, b1};
+        const int pairs[][2] = {{0, 2}};
+        return check_args(a, 10, pairs, 1);
     }
-    return true;
+    const arg_t a[] = {rows("d_x", p.d_x, p.ld_d_x, true), rows("d_u", p.d_u, p.ld_d_u, true), rows("d_gate", p.d_gate, p.ld_d_gate, true),
+                       vec("d_scale", p.d_scale, true), vec("d_w_post", p.d_w_post, true), vec("d_b_post", p.d_b_post, true),
+                       vec("d_w_pre", p.d_w_pre, true), vec("d_b_pre", p.d_b_pre, true),
+                       arg_t{"workspace", p.workspace, 4, 1, {p.workspace ? p.workspace_floats : 0}, {1}, true},
+                       rows("d_y", p.d_y, p.ld_d_y, false), rows("d_n", p.d_n, p.ld_d_n, false), x, u, g, sc, w0, b0, w1, b1};
+    const int pairs[][2] = {{0, 9}};
+    return check_args(a, 19, pairs, 1);
 }
 
-template <typename E, bool VEC, bool LN>
+template <typename E, bool LN>
 static void launch_norm(const xrl_block_norm_t& p, bool backward, hipStream_t s) {
     const int L = norm_lanes(p.D);
 #define NORM_CASE(LL)                                                                                                            \
     case LL: {                                                                                                                   \
         using G = norm_geom<LL>;                                                                                                 \
-        if (backward) hipLaunchKernelGGL((block_norm_bwd_kernel<E, LL, VEC, LN>), dim3(norm_lines(p)), dim3(G::THREADS), 0, s, p); \
+        if (backward) hipLaunchKernelGGL((block_norm_bwd_kernel<E, LL, LN>), dim3(norm_lines(p)), dim3(G::THREADS), 0, s, p); \
         else {                                                                                                                   \
             const int64_t need = (p.N + G::ROWS - 1) / G::ROWS, most = 2048 * 256 / G::THREADS;                                  \
-            hipLaunchKernelGGL((block_norm_fwd_kernel<E, LL, VEC, LN>), dim3((int)(need < most ? need : most)), dim3(G::THREADS), 0, s, p); \
+            hipLaunchKernelGGL((block_norm_fwd_kernel<E, LL, LN>), dim3((int)(need < most ? need : most)), dim3(G::THREADS), 0, s, p); \
         }                                                                                                                        \
     } break;
     switch (L) { NORM_CASE(8) NORM_CASE(16) NORM_CASE(32) NORM_CASE(64) NORM_CASE(128) NORM_CASE(256) NORM_CASE(512) NORM_CASE(1024) }
@@ -352,14 +354,9 @@ static void launch_norm(const xrl_block_norm_t& p, bool backward, hipStream_t s)
 }
 
 static int run_norm(const xrl_block_norm_t& p, bool backward, hipStream_t s) {
-    const bool vec = norm_vec(p, backward), ln = p.kind == XRL_NORM_LAYER;
-    if (p.dtype == XRL_F32) {
-        if (vec) { if (ln) launch_norm<float, true, true>(p, backward, s); else launch_norm<float, true, false>(p, backward, s); }
-        else { if (ln) launch_norm<float, false, true>(p, backward, s); else launch_norm<float, false, false>(p, backward, s); }
-    } else {
-        if (vec) { if (ln) launch_norm<bf16_t, true, true>(p, backward, s); else launch_norm<bf16_t, true, false>(p, backward, s); }
-        else { if (ln) launch_norm<bf16_t, false, true>(p, backward, s); else launch_norm<bf16_t, false, false>(p, backward, s); }
-    }
+    const bool ln = p.kind == XRL_NORM_LAYER;
+    if (p.dtype == XRL_F32) { if (ln) launch_norm<float, true>(p, backward, s); else launch_norm<float, false>(p, backward, s); }
+    else { if (ln) launch_norm<bf16_t, true>(p, backward, s); else launch_norm<bf16_t, false>(p, backward, s); }
     XRL_CHECK_LAUNCH();
     return XRL_OK;
 }
@@ -379,6 +376,7 @@ extern "C" int xrl_block_norm_forward(const xrl_block_norm_t* pp, xrl_stream_t s
     if (int rc = check_norm(p)) return rc;
     if (p.N == 0) return XRL_OK;
     XRL_CHECK_ARG(p.x && p.u && p.y);
+    if (int rc = check_norm_tensors(p, false)) return rc;
     return run_norm(p, false, as_stream(stream));
 }
 
@@ -389,6 +387,7 @@ extern "C" int xrl_block_norm_backward(const xrl_block_norm_t* pp, xrl_stream_t 
     XRL_CHECK_ARG(!p.d_gate || p.gate);
     XRL_CHECK_ARG(p.N == 0 || (p.x && p.u && p.d_x && p.d_u && (p.d_y || p.d_n) && p.workspace));
     XRL_CHECK_ARG(p.workspace_floats >= (int64_t)norm_lines(p) * NORM_SUMS * p.D);
+    if (int rc = check_norm_tensors(p, true)) return rc;
     if (p.N > 0)
         if (int rc = run_norm(p, true, as_stream(stream))) return rc;
     if (p.d_scale || p.d_w_post || p.d_b_post || p.d_w_pre || p.d_b_pre) {

@@ -5,6 +5,7 @@
 // is the forward pass for (a, b, c) = (q, k, v) and the gradients for
 //     d_q: (d_out, v, k), S_in = state^T;     d_k: (v, d_out, q) and d_v: (k, q, d_out) in reversed time, S_in = d_state_out(^T), off = 0,
 // because S_t meets d S_t exactly where o_t meets q_t.  A launch runs one job (forward) or three (backward) of it.
+#include "args.h"
 #include "linattn_mix.h"
 
 namespace xrl {
@@ -101,6 +102,31 @@ static int check_sizes(const xrl_linattn_t& p) {
 }
 
 static void set_strides(int64_t* d, const int64_t* s) { d[0] = s[0]; d[1] = s[1]; d[2] = s[2]; }
+
+static arg_t rows_arg(const char* name, const xrl_linattn_t& p, const void* ptr, const int64_t* s, int d, bool out) {
+    return arg_t{name, ptr, p.dtype == XRL_F32 ? 4 : 2, 4, {p.T, p.B, p.H, d}, {s[0], s[1], s[2], 1}, out};
+}
+static arg_t dense_arg(const char* name, const void* ptr, int64_t n, bool out) { return arg_t{name, ptr, 4, 1, {n}, {1}, out}; }
+
+static int check_tensors(const xrl_linattn_t& p, bool backward) {
+    const int64_t states = (int64_t)p.B * p.H * p.dk * p.dv;
+    const arg_t q = rows_arg("q", p, p.q, p.stride_q, p.dk, false), k = rows_arg("k", p, p.k, p.stride_k, p.dk, false),
+                v = rows_arg("v", p, p.v, p.stride_v, p.dv, false), state = dense_arg("state", p.state, states, false),
+                decay = dense_arg("log_decay", p.log_decay, p.H, false), reset = dense_arg("reset", p.reset, (int64_t)p.T * p.B, false),
+                lengths = dense_arg("lengths", p.lengths, p.B, false);
+    const int64_t ws = p.workspace ? p.workspace_floats : 0;
+    if (!backward) {
+        const arg_t a[] = {rows_arg("out", p, p.out, p.stride_out, p.dv, true), dense_arg("state_out", p.state_out, states, true),
+                           dense_arg("workspace", p.workspace, ws, true), q, k, v, state, decay, reset, lengths};
+        const int pairs[][2] = {{1, 6}};
+        return check_args(a, 10, pairs, 1);
+    }
+    const arg_t a[] = {rows_arg("d_q", p, p.d_q, p.stride_d_q, p.dk, true), rows_arg("d_k", p, p.d_k, p.stride_d_k, p.dk, true),
+                       rows_arg("d_v", p, p.d_v, p.stride_d_v, p.dv, true), dense_arg("d_state", p.d_state, states, true),
+                       dense_arg("workspace", p.workspace, ws, true), q, k, v, rows_arg("d_out", p, p.d_out, p.stride_d_out, p.dv, false),
+                       state, dense_arg("d_state_out", p.d_state_out, states, false), decay, reset, lengths};
+    return check_args(a, 14, nullptr, 0);
+}
 
 static mix_job_t forward_job(const xrl_linattn_t& p) {
     mix_job_t j{};
@@ -224,6 +250,7 @@ extern "C" int xrl_linattn_forward(const xrl_linattn_t* pp, xrl_stream_t stream)
     if (int rc = check_sizes(p)) return rc;
     XRL_CHECK_ARG(p.log_decay && (p.T == 0 || p.B == 0 || (p.q && p.k && p.v && p.out)));
     if (p.B == 0) return XRL_OK;
+    if (int rc = check_tensors(p, false)) return rc;
     const int64_t need = xrl_linattn_workspace_floats(pp, 0);
     XRL_CHECK_ARG(need == 0 || (p.workspace && p.workspace_floats >= need));
     mix_t m{};
@@ -237,8 +264,8 @@ extern "C" int xrl_linattn_backward(const xrl_linattn_t* pp, xrl_stream_t stream
     const xrl_linattn_t& p = *pp;
     if (int rc = check_sizes(p)) return rc;
     XRL_CHECK_ARG(p.log_decay && (p.T == 0 || p.B == 0 || (p.q && p.k && p.v && p.d_out && p.d_q && p.d_k && p.d_v)));
-    XRL_CHECK_ARG(!p.d_state || p.d_state != p.d_state_out);         // d_k's job reads d_state_out while d_v's writes d_state
     if (p.B == 0) return XRL_OK;
+    if (int rc = check_tensors(p, true)) return rc;                  // d_state is not d_state_out: d_k's job reads it while d_v's writes
     const int64_t need = xrl_linattn_workspace_floats(pp, 1);
     XRL_CHECK_ARG(need == 0 || (p.workspace && p.workspace_floats >= need));
     mix_t m{};
@@ -254,6 +281,7 @@ extern "C" int xrl_linattn_step(const xrl_linattn_t* pp, xrl_stream_t stream) {
     XRL_CHECK_ARG(p.T == 1);
     if (p.B == 0) return XRL_OK;
     XRL_CHECK_ARG(p.q && p.k && p.v && p.out && p.log_decay && p.state && p.state_out);
+    if (int rc = check_tensors(p, false)) return rc;
     const bool vec = p.dv % 4 == 0 && ((reinterpret_cast<uintptr_t>(p.state) | reinterpret_cast<uintptr_t>(p.state_out)) & 15) == 0;
     const int threads = 256;
     const dim3 grid(p.B * p.H);

@@ -5,12 +5,13 @@ current HIP stream to libxrl_hip.so, and returns nothing: outputs are written in
 of them may be recorded into a hipGraph (xuance_amd.graph.Graph).
 """
 import ctypes as C
+import struct
 
 import torch
 
 from . import _lib
 from ._lib import XrlError  # noqa: F401  (re-exported)
-from ._lib import (ActTail, MlpChain, Conv, ImageJob, DqnHeadTd, DqnTailTd, DqnActTail, Classic, Exchange, MarlGate, SynthMarl, SynthFrames, LstmFwd, LstmBwd, EpisodeField, GruFwd, GruBwd, Mirrors, RolloutRun, RolloutWide, SynthCtl, ACT, Field, Gemm, PpoLoss, AdamState, Rms, Sample, CartPole, PostStep, EGreedy, DqnTd, Qmix, RolloutStep, FusedLayer, PpoFused, OptChain, CHAIN_SYNC_WORDS, MarlAct, LinAttn, BlockNorm, Distill, call, ptr,
+from ._lib import (ActTail, MlpChain, Conv, ImageJob, DqnHeadTd, DqnTailTd, DqnActTail, Classic, Exchange, MarlGate, SynthMarl, SynthFrames, LstmFwd, LstmBwd, EpisodeField, GruFwd, GruBwd, Mirrors, RolloutRun, RolloutWide, SynthCtl, ACT, Field, Gemm, PpoLoss, AdamState, Rms, Sample, CartPole, PostStep, EGreedy, DqnTd, Qmix, RolloutStep, FusedLayer, PpoFused, OptChain, CHAIN_SYNC_WORDS, MarlAct, call, ptr,
                    stream_ptr)
 
 
@@ -1211,8 +1212,14 @@ def gru_backward(**kw):
 
 
 # ------------------------------------------------------------------------------------------ sequence policies
+# The structs are packed in one go (their layouts: _lib.LinAttn, BlockNorm, Distill): an acting step is a launch of microseconds, and setting
+# fifty ctypes fields one by one takes as long.
+_LINATTN = struct.Struct("@16Pq24q6ifi")
+_BLOCK_NORM = struct.Struct("@21P12q4ifi")
+_DISTILL = struct.Struct("@7P3q3iffi")
 _IO_DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 NORM_KIND = {"rms": 0, "layer": 1}
+_ROWS0 = (0, 0, 0)
 
 
 def _need(cond, what):
@@ -1221,66 +1228,34 @@ def _need(cond, what):
 
 
 def _on_device(t, device):
-    return t.is_cuda and t.device.index == device
+    return t.get_device() == device
 
 
-def _arg(name, t, shape, dtype, device, dense=False):
-    """One tensor of a call: on the current device, of this shape and type, its last dimension contiguous (dense: all of them)."""
-    if t is None:
-        return
+def _wrong(name, t, shape, dtype, device):
     if not _on_device(t, device):
         raise XrlError(f"{name}: needs a tensor on the current device cuda:{device}, got {t.device}")
-    if t.dtype is not dtype or tuple(t.shape) != tuple(shape):
-        raise XrlError(f"{name}: needs {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
-    if dense:
-        if not t.is_contiguous():
-            raise XrlError(f"{name}: has to be contiguous, strides are {t.stride()}")
-    elif t.shape[-1] > 1 and t.stride(-1) != 1:
-        raise XrlError(f"{name}: its last dimension has to be contiguous, strides are {t.stride()}")
+    raise XrlError(f"{name}: needs {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
 
 
-def _output(name, t):
-    """Every element of an output has a place of its own: strides, largest first, each pass what the ones below it span."""
-    if t is None or t.numel() == 0 or t.is_contiguous():
-        return
-    span = 1
-    for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n > 1):
-        _need(st >= span, f"{name}: is written to and its elements share memory, strides are {t.stride()} for {tuple(t.shape)}")
-        span = st * (n - 1) + span
+def _dense(name, t, shape, dtype, device):
+    """-> address of a contiguous tensor (0: None) on the current device."""
+    if t is None:
+        return 0
+    if not _on_device(t, device) or t.dtype is not dtype or t.shape != shape:
+        _wrong(name, t, shape, dtype, device)
+    if not t.is_contiguous():
+        raise XrlError(f"{name}: has to be contiguous, strides are {t.stride()}")
+    return t.data_ptr()
 
 
-def _extent(t):
-    """first and last byte + 1 that a tensor's elements lie in"""
-    n = sum(st * (s - 1) for st, s in zip(t.stride(), t.shape)) + 1
-    return t.data_ptr(), t.data_ptr() + n * t.element_size()
-
-
-def _interleaved(t, u):
-    """Two tensors over the same stretch of memory without a common element: slices of one wider row, the rows at the same pitch."""
-    if t.dim() != u.dim() or t.element_size() != u.element_size():
-        return False
-    for inner in range(1, t.dim()):
-        outer = [(t.stride(i), u.stride(i)) for i in range(t.dim() - inner) if t.shape[i] > 1 or u.shape[i] > 1]
-        pitch = min((a for a, _ in outer), default=0)
-        if pitch <= 0 or any(a != b or a % pitch for a, b in outer):
-            continue
-        spans = [sum(x.stride(i) * (x.shape[i] - 1) for i in range(x.dim() - inner, x.dim())) + 1 for x in (t, u)]
-        off, rest = divmod(u.data_ptr() - t.data_ptr(), t.element_size())
-        off %= pitch
-        if rest == 0 and off >= spans[0] and off + spans[1] <= pitch:
-            return True
-    return False
-
-
-def _apart(outs, ins, pairs=()):
-    """No output shares memory with another tensor of the call; pairs: (output, input) names that may be the very same tensor."""
-    both = [(k, t, *_extent(t)) for d in (outs, ins) for k, t in d.items() if t is not None and t.numel()]
-    for i, (o, t, lo, hi) in enumerate(both):
-        if o not in outs:
-            break
-        for k, u, a, b in both[i + 1:]:
-            if b > lo and hi > a and not ((o, k) in pairs and lo == a and t.stride() == u.stride()) and not _interleaved(t, u):
-                raise XrlError(f"{o} and {k} share memory")
+def _rows(name, t, shape, dtype, device):
+    """-> address and strides of a tensor on the current device whose last dimension is contiguous."""
+    if not _on_device(t, device) or t.dtype is not dtype or t.shape != shape:
+        _wrong(name, t, shape, dtype, device)
+    st = t.stride()
+    if st[-1] != 1 and shape[-1] > 1:
+        raise XrlError(f"{name}: its last dimension has to be contiguous, strides are {st}")
+    return t.data_ptr(), st[:-1]
 
 
 def _io_dtype(t):
@@ -1291,57 +1266,28 @@ def _io_dtype(t):
 def _workspace(given, floats, device):
     """The caller's workspace, or one from the allocator.  While a graph is captured it has to be the caller's: the graph keeps its
     address, and two graphs that may run at the same time need one each."""
-    if floats == 0:
-        return None
+    _lib.check(min(floats, 0), "workspace")
     if given is None:
         _need(not torch.cuda.is_current_stream_capturing(), f"a captured call needs workspace=, a float32 tensor of {floats} elements")
         return torch.empty(floats, device=f"cuda:{device}")
-    _need(_on_device(given, device) and given.dtype == torch.float32 and given.is_contiguous() and given.numel() >= floats
-          and given.data_ptr() % 16 == 0, f"workspace: needs {floats} contiguous, 16-byte aligned float32 elements on cuda:{device}")
+    _need(_on_device(given, device) and given.dtype is torch.float32 and given.is_contiguous() and given.numel() >= floats and
+          given.data_ptr() % 16 == 0, f"workspace: needs {floats} contiguous, 16-byte aligned float32 elements on cuda:{device}")
     return given
-
-
-def _linattn(q, k, v, log_decay, scale, lengths, reset, state, state_out):
-    init_device()
-    p = LinAttn()
-    _need(q.dim() == 4 and v.dim() == 4, f"q, k, v: [T, B, H, d] each, got {tuple(q.shape)}, {tuple(v.shape)}")
-    dev = torch.cuda.current_device()
-    T, B, H, dk = q.shape
-    dv, dt = v.shape[-1], q.dtype
-    p.dtype = _io_dtype(q)
-    _need(1 <= dk <= 128 and 1 <= dv <= 128, f"head dimensions 1..128, got {dk} and {dv}")
-    for name, t, d in (("q", q, dk), ("k", k, dk), ("v", v, dv)):
-        _arg(name, t, (T, B, H, d), dt, dev)
-        setattr(p, name, t.data_ptr())
-        st = t.stride()
-        _need(min(st[:3]) >= 0, f"{name}: negative strides")
-        getattr(p, "stride_" + name)[:] = st[:3]
-    _arg("log_decay", log_decay, (H,), torch.float32, dev, True)
-    _arg("lengths", lengths, (B,), torch.int32, dev, True)
-    _arg("reset", reset, (T, B), torch.float32, dev, True)
-    _arg("state", state, (B, H, dk, dv), torch.float32, dev, True)
-    _arg("state_out", state_out, (B, H, dk, dv), torch.float32, dev, True)
-    p.log_decay, p.lengths, p.reset, p.state, p.state_out = ptr(log_decay), ptr(lengths), ptr(reset), ptr(state), ptr(state_out)
-    p.T, p.B, p.H, p.dk, p.dv, p.scale = T, B, H, dk, dv, float(scale)
-    return p, dev
-
-
-def _linattn_io(p, dev, dtype, **tensors):
-    for name, (t, d, out) in tensors.items():
-        _arg(name, t, (p.T, p.B, p.H, d), dtype, dev)
-        if out:
-            _output(name, t)
-        setattr(p, name, t.data_ptr())
-        getattr(p, "stride_" + name)[:] = t.stride()[:3]
 
 
 def linattn_workspace_floats(T, B, H, dk, dv, backward=False, dtype=torch.float32):
     """Floats of workspace that linattn_forward / linattn_backward need at these sizes (0: none)."""
-    p = LinAttn()
-    p.T, p.B, p.H, p.dk, p.dv, p.dtype = int(T), int(B), int(H), int(dk), int(dv), _IO_DTYPES[dtype]
-    n = _lib.load().xrl_linattn_workspace_floats(C.byref(p), int(bool(backward)))
+    p = _LINATTN.pack(*(0,) * 41, int(T), int(B), int(H), int(dk), int(dv), _IO_DTYPES[dtype], 1.0, 0)
+    n = _lib.load().xrl_linattn_workspace_floats(p, int(bool(backward)))
     _lib.check(min(n, 0), "xrl_linattn_workspace_floats")
     return n
+
+
+def _linattn_sizes(q, v):
+    init_device()
+    if q.dim() != 4 or v.dim() != 4:
+        raise XrlError(f"q, k, v: [T, B, H, d] each, got {tuple(q.shape)}, {tuple(v.shape)}")
+    return (*q.shape, v.shape[3], _io_dtype(q), torch.cuda.current_device())
 
 
 def linattn_forward(q, k, v, out, log_decay, scale=1.0, lengths=None, reset=None, state=None, state_out=None, workspace=None):
@@ -1351,13 +1297,22 @@ def linattn_forward(q, k, v, out, log_decay, scale=1.0, lengths=None, reset=None
     projection, expanded heads), the last dimension contiguous, dk and dv up to 128.  log_decay [H] <= 0 (-inf: no memory), lengths [B]
     int32: the steps at and behind a row's length are not read and their outputs are 0.  reset [T, B], state / state_out [B, H, dk, dv]
     float32 (state_out may be state): S before the first and after the last step.  Inputs have to be finite."""
-    p, dev = _linattn(q, k, v, log_decay, scale, lengths, reset, state, state_out)
-    _linattn_io(p, dev, q.dtype, out=(out, p.dv, True))
-    _apart({"out": out, "state_out": state_out}, {"q": q, "k": k, "v": v, "state": state}, {("state_out", "state")})
-    ws = _workspace(workspace, _lib.load().xrl_linattn_workspace_floats(C.byref(p), 0), dev)
-    if ws is not None:
-        p.workspace, p.workspace_floats = ws.data_ptr(), ws.numel()
-    call("xrl_linattn_forward", C.byref(p), stream_ptr())
+    T, B, H, dk, dv, dt, dev = _linattn_sizes(q, v)
+    f32, typ, ks, vs, ss = torch.float32, q.dtype, (T, B, H, dk), (T, B, H, dv), (B, H, dk, dv)
+    pq, sq = _rows("q", q, ks, typ, dev)
+    pk, sk = _rows("k", k, ks, typ, dev)
+    pv, sv = _rows("v", v, vs, typ, dev)
+    po, so = _rows("out", out, vs, typ, dev)
+    ptrs = (pq, pk, pv, po, _dense("log_decay", log_decay, (H,), f32, dev), _dense("lengths", lengths, (B,), torch.int32, dev),
+            _dense("reset", reset, (T, B), f32, dev), _dense("state", state, ss, f32, dev), _dense("state_out", state_out, ss, f32, dev),
+            0, 0, 0, 0, 0, 0)
+    rest = (*sq, *sk, *sv, *so, *_ROWS0, *_ROWS0, *_ROWS0, *_ROWS0, T, B, H, dk, dv, dt, scale, 0)
+    p = _LINATTN.pack(*ptrs, 0, 0, *rest)
+    need = _lib.load().xrl_linattn_workspace_floats(p, 0)
+    if need:
+        ws = _workspace(workspace, need, dev)
+        p = _LINATTN.pack(*ptrs, ws.data_ptr(), ws.numel(), *rest)
+    call("xrl_linattn_forward", p, stream_ptr())
 
 
 def linattn_backward(q, k, v, d_out, d_q, d_k, d_v, log_decay, scale=1.0, lengths=None, reset=None, state=None, d_state_out=None,
@@ -1365,54 +1320,59 @@ def linattn_backward(q, k, v, d_out, d_q, d_k, d_v, log_decay, scale=1.0, length
     """Gradients of linattn_forward (xrl_linattn_backward): d_q, d_k, d_v and, where given, d_state, from d_out and d_state_out (None: 0).
     Nothing is kept from the forward pass.  log_decay is a constant of the head.  Of inputs with shared heads (stride 0) the gradients come
     per head, to be summed by the caller."""
-    p, dev = _linattn(q, k, v, log_decay, scale, lengths, reset, state, None)
-    _linattn_io(p, dev, q.dtype, d_out=(d_out, p.dv, False), d_q=(d_q, p.dk, True), d_k=(d_k, p.dk, True), d_v=(d_v, p.dv, True))
-    for name, t in (("d_state_out", d_state_out), ("d_state", d_state)):
-        _arg(name, t, (p.B, p.H, p.dk, p.dv), torch.float32, dev, True)
-    p.d_state_out, p.d_state = ptr(d_state_out), ptr(d_state)
-    _apart({"d_q": d_q, "d_k": d_k, "d_v": d_v, "d_state": d_state},
-           {"q": q, "k": k, "v": v, "d_out": d_out, "state": state, "d_state_out": d_state_out})
-    ws = _workspace(workspace, _lib.load().xrl_linattn_workspace_floats(C.byref(p), 1), dev)
-    if ws is not None:
-        p.workspace, p.workspace_floats = ws.data_ptr(), ws.numel()
-    call("xrl_linattn_backward", C.byref(p), stream_ptr())
+    T, B, H, dk, dv, dt, dev = _linattn_sizes(q, v)
+    f32, typ, ks, vs, ss = torch.float32, q.dtype, (T, B, H, dk), (T, B, H, dv), (B, H, dk, dv)
+    pq, sq = _rows("q", q, ks, typ, dev)
+    pk, sk = _rows("k", k, ks, typ, dev)
+    pv, sv = _rows("v", v, vs, typ, dev)
+    pdo, sdo = _rows("d_out", d_out, vs, typ, dev)
+    pdq, sdq = _rows("d_q", d_q, ks, typ, dev)
+    pdk, sdk = _rows("d_k", d_k, ks, typ, dev)
+    pdv, sdv = _rows("d_v", d_v, vs, typ, dev)
+    ptrs = (pq, pk, pv, 0, _dense("log_decay", log_decay, (H,), f32, dev), _dense("lengths", lengths, (B,), torch.int32, dev),
+            _dense("reset", reset, (T, B), f32, dev), _dense("state", state, ss, f32, dev), 0, pdo, pdq, pdk, pdv,
+            _dense("d_state_out", d_state_out, ss, f32, dev), _dense("d_state", d_state, ss, f32, dev))
+    rest = (*sq, *sk, *sv, *_ROWS0, *sdo, *sdq, *sdk, *sdv, T, B, H, dk, dv, dt, scale, 0)
+    p = _LINATTN.pack(*ptrs, 0, 0, *rest)
+    need = _lib.load().xrl_linattn_workspace_floats(p, 1)
+    if need:
+        ws = _workspace(workspace, need, dev)
+        p = _LINATTN.pack(*ptrs, ws.data_ptr(), ws.numel(), *rest)
+    call("xrl_linattn_backward", p, stream_ptr())
 
 
 def linattn_step(q, k, v, out, log_decay, state, state_out=None, scale=1.0, reset=None):
     """One acting step (xrl_linattn_step): q, k [B, H, dk], v, out [B, H, dv], reset [B]; state [B, H, dk, dv] float32 is carried on in place, or
     into state_out."""
-    _need(q.dim() == 3 and v.dim() == 3 and k.dim() == 3 and out.dim() == 3, "q, k, v, out: [B, H, d] each")
-    if state_out is None:
-        state_out = state
-    p, dev = _linattn(q.unsqueeze(0), k.unsqueeze(0), v.unsqueeze(0), log_decay, scale, None, None if reset is None else reset.unsqueeze(0),
-                      state, state_out)
-    _linattn_io(p, dev, q.dtype, out=(out.unsqueeze(0), p.dv, True))
-    _apart({"out": out, "state_out": state_out}, {"q": q, "k": k, "v": v, "state": state}, {("state_out", "state")})
-    call("xrl_linattn_step", C.byref(p), stream_ptr())
+    if q.dim() != 3 or v.dim() != 3:
+        raise XrlError(f"q, k, v: [B, H, d] each, got {tuple(q.shape)}, {tuple(v.shape)}")
+    B, H, dk = q.shape
+    dv, dt, dev = v.shape[2], _io_dtype(q), torch.cuda.current_device()
+    f32, typ, ks, vs, ss = torch.float32, q.dtype, (B, H, dk), (B, H, dv), (B, H, dk, dv)
+    pq, sq = _rows("q", q, ks, typ, dev)
+    pk, sk = _rows("k", k, ks, typ, dev)
+    pv, sv = _rows("v", v, vs, typ, dev)
+    po, so = _rows("out", out, vs, typ, dev)
+    ps = _dense("state", state, ss, f32, dev)
+    pn = ps if state_out is None else _dense("state_out", state_out, ss, f32, dev)
+    p = _LINATTN.pack(pq, pk, pv, po, _dense("log_decay", log_decay, (H,), f32, dev), 0, _dense("reset", reset, (B,), f32, dev), ps, pn,
+                      0, 0, 0, 0, 0, 0, 0, 0, 0, *sq, 0, *sk, 0, *sv, 0, *so, *_ROWS0, *_ROWS0, *_ROWS0, *_ROWS0, 1, B, H, dk, dv, dt, scale, 0)
+    call("xrl_linattn_step", p, stream_ptr())
 
 
-_NORM_VECTORS = ("scale", "w_post", "b_post", "w_pre", "b_pre")
+def _norm_args(x, kind, gate_act, eps):
+    if x.dim() != 2:
+        raise XrlError(f"x: [N, D], got {tuple(x.shape)}")
+    if kind not in NORM_KIND or gate_act not in ACT or not eps > 0:
+        raise XrlError(f"kind {kind!r} of {sorted(NORM_KIND)}, gate_act {gate_act!r} of the activations, eps {eps} > 0")
+    return x.shape, (x.shape[1],), x.dtype, _io_dtype(x), torch.cuda.current_device()
 
 
-def _block_norm(x, kind, gate_act, eps, rows, vectors):
-    p = BlockNorm()
-    _need(x.dim() == 2, f"x: [N, D], got {tuple(x.shape)}")
-    _need(kind in NORM_KIND and gate_act in ACT and eps > 0, f"kind {kind!r} of {sorted(NORM_KIND)}, gate_act {gate_act!r} of the activations, eps {eps} > 0")
-    dev = torch.cuda.current_device()
-    N, D = x.shape
-    p.dtype, p.kind, p.gate_act, p.eps, p.N, p.D = _io_dtype(x), NORM_KIND[kind], ACT[gate_act], float(eps), N, D
-    _need(1 <= D <= 8192, f"rows of 1..8192 values, got {D}")
-    for name, t in rows.items():
-        if t is not None:
-            _arg(name, t, (N, D), x.dtype, dev)
-            setattr(p, name, t.data_ptr())
-            setattr(p, "ld_" + name, t.stride(0))
-            _need(t.stride(0) >= 0, f"{name}: negative strides")
-    for name, t in vectors.items():
-        if t is not None:
-            _arg(name, t, (D,), torch.float32, dev, True)
-            setattr(p, name, t.data_ptr())
-    return p, dev
+def _opt_rows(name, t, shape, dtype, device):
+    if t is None:
+        return 0, 0
+    p, st = _rows(name, t, shape, dtype, device)
+    return p, st[0]
 
 
 def block_norm_forward(x, u, y, n=None, gate=None, gate_act="sigmoid", scale=None, w_post=None, b_post=None, w_pre=None, b_pre=None,
@@ -1421,19 +1381,23 @@ def block_norm_forward(x, u, y, n=None, gate=None, gate_act="sigmoid", scale=Non
         y = x + scale * act(gate) * (norm(u) * w_post + b_post),    n = norm(y) * w_pre + b_pre
     x (residual stream), u (output of the block), gate, y (stream after it), n (input of the next block): [N, D] float32 or bfloat16,
     D up to 8192, rows of any stride; scale, weights, biases [D] float32, a missing one is 1 or 0.  kind "rms" or "layer".  y may be x."""
-    p, dev = _block_norm(x, kind, gate_act, eps, dict(x=x, u=u, gate=gate, y=y, n=n),
-                         dict(scale=scale, w_post=w_post, b_post=b_post, w_pre=w_pre, b_pre=b_pre))
-    _output("y", y)
-    _output("n", n)
-    _apart({"y": y, "n": n}, {"x": x, "u": u, "gate": gate}, {("y", "x")})
-    call("xrl_block_norm_forward", C.byref(p), stream_ptr())
+    shape, vec, typ, dt, dev = _norm_args(x, kind, gate_act, eps)
+    f32 = torch.float32
+    px, lx = _opt_rows("x", x, shape, typ, dev)
+    pu, lu = _opt_rows("u", u, shape, typ, dev)
+    pg, lg = _opt_rows("gate", gate, shape, typ, dev)
+    py, ly = _opt_rows("y", y, shape, typ, dev)
+    pn, ln = _opt_rows("n", n, shape, typ, dev)
+    p = _BLOCK_NORM.pack(px, pu, pg, py, pn, _dense("scale", scale, vec, f32, dev), _dense("w_post", w_post, vec, f32, dev),
+                         _dense("b_post", b_post, vec, f32, dev), _dense("w_pre", w_pre, vec, f32, dev), _dense("b_pre", b_pre, vec, f32, dev),
+                         0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, shape[0], lx, lu, lg, ly, ln, 0, 0, 0, 0, 0, shape[1], dt, NORM_KIND[kind],
+                         ACT[gate_act], eps, 0)
+    call("xrl_block_norm_forward", p, stream_ptr())
 
 
 def block_norm_workspace_floats(N, D, dtype=torch.float32):
     """Floats of workspace that block_norm_backward needs for N rows of D values."""
-    p = BlockNorm()
-    p.N, p.D, p.dtype, p.eps = int(N), int(D), _IO_DTYPES[dtype], 1e-5
-    n = _lib.load().xrl_block_norm_workspace_floats(C.byref(p))
+    n = _lib.load().xrl_block_norm_workspace_floats(_BLOCK_NORM.pack(*(0,) * 22, int(N), *(0,) * 10, int(D), _IO_DTYPES[dtype], 0, 0, 1e-5, 0))
     _lib.check(min(n, 0), "xrl_block_norm_workspace_floats")
     return n
 
@@ -1444,19 +1408,27 @@ def block_norm_backward(x, u, d_y, d_n, d_x, d_u, d_gate=None, d_scale=None, d_w
     """Gradients of block_norm_forward (xrl_block_norm_backward) from d_y and d_n (either may be None: 0): d_x, d_u, where given d_gate
     [N, D] and the sums over the rows d_scale, d_w_post, d_b_post, d_w_pre, d_b_pre [D] float32.  Needs x, u and gate of the forward pass,
     nothing else; the order of the sums is fixed.  d_x may be d_y."""
-    sums = dict(d_scale=d_scale, d_w_post=d_w_post, d_b_post=d_b_post, d_w_pre=d_w_pre, d_b_pre=d_b_pre)
-    p, dev = _block_norm(x, kind, gate_act, eps, dict(x=x, u=u, gate=gate, d_y=d_y, d_n=d_n, d_x=d_x, d_u=d_u, d_gate=d_gate),
-                         dict(scale=scale, w_post=w_post, b_post=b_post, w_pre=w_pre, b_pre=b_pre, **sums))
-    _need(d_gate is None or gate is not None, "d_gate without a gate")
-    _need(d_y is not None or d_n is not None, "neither d_y nor d_n")
-    for name, t in (("d_x", d_x), ("d_u", d_u), ("d_gate", d_gate)):
-        _output(name, t)
-    _apart({"d_x": d_x, "d_u": d_u, "d_gate": d_gate, **sums},
-           {"x": x, "u": u, "gate": gate, "d_y": d_y, "d_n": d_n, "scale": scale, "w_post": w_post, "b_post": b_post, "w_pre": w_pre}, {("d_x", "d_y")})
-    ws = _workspace(workspace, _lib.load().xrl_block_norm_workspace_floats(C.byref(p)), dev)
-    if ws is not None:
-        p.workspace, p.workspace_floats = ws.data_ptr(), ws.numel()
-    call("xrl_block_norm_backward", C.byref(p), stream_ptr())
+    shape, vec, typ, dt, dev = _norm_args(x, kind, gate_act, eps)
+    f32 = torch.float32
+    px, lx = _opt_rows("x", x, shape, typ, dev)
+    pu, lu = _opt_rows("u", u, shape, typ, dev)
+    pg, lg = _opt_rows("gate", gate, shape, typ, dev)
+    pdy, ldy = _opt_rows("d_y", d_y, shape, typ, dev)
+    pdn, ldn = _opt_rows("d_n", d_n, shape, typ, dev)
+    pdx, ldx = _opt_rows("d_x", d_x, shape, typ, dev)
+    pdu, ldu = _opt_rows("d_u", d_u, shape, typ, dev)
+    pdg, ldg = _opt_rows("d_gate", d_gate, shape, typ, dev)
+    ptrs = (px, pu, pg, 0, 0, _dense("scale", scale, vec, f32, dev), _dense("w_post", w_post, vec, f32, dev), _dense("b_post", b_post, vec, f32, dev),
+            _dense("w_pre", w_pre, vec, f32, dev), _dense("b_pre", b_pre, vec, f32, dev), pdy, pdn, pdx, pdu, pdg,
+            _dense("d_scale", d_scale, vec, f32, dev), _dense("d_w_post", d_w_post, vec, f32, dev), _dense("d_b_post", d_b_post, vec, f32, dev),
+            _dense("d_w_pre", d_w_pre, vec, f32, dev), _dense("d_b_pre", d_b_pre, vec, f32, dev))
+    rest = (shape[0], lx, lu, lg, 0, 0, ldy, ldn, ldx, ldu, ldg, shape[1], dt, NORM_KIND[kind], ACT[gate_act], eps, 0)
+    need = _lib.load().xrl_block_norm_workspace_floats(_BLOCK_NORM.pack(*ptrs, 0, 0, *rest))
+    ws = (0, 0)
+    if need:
+        buf = _workspace(workspace, need, dev)
+        ws = (buf.data_ptr(), buf.numel())
+    call("xrl_block_norm_backward", _BLOCK_NORM.pack(*ptrs, *ws, *rest), stream_ptr())
 
 
 def distill_loss(logits, teacher_idx, teacher_logits, loss, d_logits=None, avail=None, weight=None, temperature=1.0, grad_scale=1.0):
@@ -1466,30 +1438,17 @@ def distill_loss(logits, teacher_idx, teacher_logits, loss, d_logits=None, avail
     logits, d_logits [N, A] float32 or bfloat16 with rows of any stride (d_logits may be logits), teacher_idx [N, K] int32 (outside 0..A-1:
     no entry), teacher_logits [N, K] of the type of logits, K up to 256, avail [N, A] float32 0/1, weight [N] float32.  A row without a
     valid teacher entry, without an available logit or of weight 0 has loss 0 and gradient 0."""
-    p = Distill()
-    _need(logits.dim() == 2 and teacher_idx.dim() == 2, "logits: [N, A], teacher_idx: [N, K]")
-    dev = torch.cuda.current_device()
-    N, A = logits.shape
+    if logits.dim() != 2 or teacher_idx.dim() != 2:
+        raise XrlError("logits: [N, A], teacher_idx: [N, K]")
+    dev, typ, f32 = torch.cuda.current_device(), logits.dtype, torch.float32
+    shape = N, A = logits.shape
     K = teacher_idx.shape[1]
-    _need(A >= 1 and 1 <= K <= 256, f"1..256 teacher entries a row and at least one action, got K = {K}, A = {A}")
-    _need(temperature > 0, f"temperature {temperature} > 0")
-    p.dtype = _io_dtype(logits)
-    _arg("logits", logits, (N, A), logits.dtype, dev)
-    _arg("teacher_idx", teacher_idx, (N, K), torch.int32, dev, True)
-    _arg("teacher_logits", teacher_logits, (N, K), logits.dtype, dev, True)
-    _arg("loss", loss, (N,), torch.float32, dev, True)
-    _arg("d_logits", d_logits, (N, A), logits.dtype, dev)
-    _arg("avail", avail, (N, A), torch.float32, dev, True)
-    _arg("weight", weight, (N,), torch.float32, dev, True)
-    _need(logits.stride(0) >= 0, "logits: negative strides")
-    _output("d_logits", d_logits)
-    _apart({"loss": loss, "d_logits": d_logits}, {"logits": logits, "teacher_idx": teacher_idx, "teacher_logits": teacher_logits,
-                                                  "avail": avail, "weight": weight}, {("d_logits", "logits")})
-    p.logits, p.teacher_idx, p.teacher_logits, p.avail, p.weight = (ptr(t) for t in (logits, teacher_idx, teacher_logits, avail, weight))
-    p.loss, p.d_logits, p.N, p.A, p.K = ptr(loss), ptr(d_logits), N, A, K
-    p.ld, p.ld_d = logits.stride(0), 0 if d_logits is None else d_logits.stride(0)
-    p.temperature, p.grad_scale = float(temperature), float(grad_scale)
-    call("xrl_distill_loss", C.byref(p), stream_ptr())
+    ps, ld = _opt_rows("logits", logits, shape, typ, dev)
+    pd, ldd = _opt_rows("d_logits", d_logits, shape, typ, dev)
+    p = _DISTILL.pack(ps, _dense("teacher_idx", teacher_idx, (N, K), torch.int32, dev), _dense("teacher_logits", teacher_logits, (N, K), typ, dev),
+                      _dense("avail", avail, shape, f32, dev), _dense("weight", weight, (N,), f32, dev), _dense("loss", loss, (N,), f32, dev), pd,
+                      N, ld, ldd, A, K, _io_dtype(logits), temperature, grad_scale, 0)
+    call("xrl_distill_loss", p, stream_ptr())
 
 
 def sync_target(params, target, P, state, sync_frequency):
