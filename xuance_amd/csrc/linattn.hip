@@ -155,16 +155,6 @@ static void backward_jobs(const xrl_linattn_t& p, mix_job_t* j) {
     v.reverse = 1; v.off = 0; v.scale_p = v.scale_b = p.scale; v.scale_s = 1.f;
 }
 
-static bool rows16(const void* p, const int64_t* s, int d, int unit, int bytes) {
-    return d % unit == 0 && s[0] % unit == 0 && s[1] % unit == 0 && s[2] % unit == 0 && reinterpret_cast<uintptr_t>(p) % bytes == 0;
-}
-
-static void set_vec(mix_job_t& j, int dtype) {
-    const int unit = dtype == XRL_F32 ? 4 : 8;
-    j.vec = (rows16(j.a, j.sa, j.da, unit, 16) ? 1 : 0) | (rows16(j.b, j.sb, j.da, unit, 16) ? 2 : 0) | (rows16(j.c, j.sc, j.dc, unit, 16) ? 4 : 0) |
-            (rows16(j.out, j.so, j.dc, 4, dtype == XRL_F32 ? 16 : 8) ? 8 : 0);
-}
-
 // Segments of the time axis: where rows x heads x jobs are too few workgroups for the chip, the axis is cut so that about two per compute unit
 // run, four chunks each at least (a segment reads b and c twice: once for its state, once for its outputs).
 static int segments(const xrl_linattn_t& p, int n_jobs, int* seg_chunks) {
@@ -195,7 +185,7 @@ static int run_jobs(const xrl_linattn_t& p, mix_t& m, int n_jobs, const int* hol
     m.log_decay = p.log_decay; m.lengths = p.lengths; m.reset = p.reset;
     m.T = p.T; m.B = p.B; m.H = p.H; m.kv = p.dk * p.dv; m.n_jobs = n_jobs;
     m.n_seg = segments(p, n_jobs, &m.seg_chunks);
-    for (int i = 0; i < n_jobs; ++i) { set_vec(m.job[i], p.dtype); m.job[i].s_row = m.kv; }
+    for (int i = 0; i < n_jobs; ++i) m.job[i].s_row = m.kv;
     if (m.n_seg == 1) return launch(p, m, s);
     mix_t st = m;
     scan_t sc{};

@@ -26,7 +26,6 @@ struct mix_job_t {
     int sd, se;
     int64_t s_row;                        // s_in: from row and head (and segment) to the next
     int reverse, off;
-    int vec;                              // bit 0 a, 1 b, 2 c, 3 out: rows allow 16-byte (out: 4-element) accesses
     float scale_p, scale_s, scale_b;      // of the products a.b, of a S, of b (x) c in the state
     float* carry;                         // pass over the states of segments: what a segment multiplies the state by
 };
@@ -34,7 +33,7 @@ struct mix_t {
     mix_job_t job[3];
     const float* log_decay; const int32_t* lengths; const float* reset;
     int T, B, H, kv;
-    int n_jobs, n_seg, seg_chunks;
+    int n_jobs, n_seg, seg_chunks, n_slices;
     int states_only;                      // write every segment's own state to s_out [row and head][segment] and its carry
 };
 
@@ -42,8 +41,10 @@ constexpr int CH = 64;                    // steps of a chunk
 
 template <typename E> struct mix_ops;
 
+// Operands by fragments: KB values of k of 16 rows or columns.  A product of fragments takes STEPS matrix instructions; an f32 operand that is made
+// here (P, the state, the weighted c) takes P_PARTS, S_PARTS, W_PARTS fragments.
 template <> struct mix_ops<float> {
-    static constexpr int KB = 16, PAD = 4, PLANES = 1;          // k of one operand fragment, row padding in LDS, planes of P
+    static constexpr int KB = 16, PAD = 4, STEPS = 4, P_PARTS = 1, S_PARTS = 1, W_PARTS = 1;
     typedef f32x4_t frag;
     // four values of a row of LDS, k = 16 p + 4 g + r
     static __device__ __forceinline__ frag row(const float* r, int p, int g) { return *reinterpret_cast<const f32x4_t*>(r + 16 * p + 4 * g); }
@@ -54,36 +55,21 @@ template <> struct mix_ops<float> {
         const f32x4_t v = {at[0], at[stride], at[2 * stride], at[3 * stride]};
         return v;
     }
-    static __device__ __forceinline__ f32x4_t mfma(frag a, frag b, f32x4_t c) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r], b[r], c, 0, 0, 0);
-        return c;
+    static __device__ __forceinline__ f32x4_t mfma(frag a, frag b, f32x4_t c, int step) {
+        return __builtin_amdgcn_mfma_f32_16x16x4f32(a[step], b[step], c, 0, 0, 0);
     }
-    // (state tiles as returned) x row fragment
-    static __device__ __forceinline__ f32x4_t mfma_state(const f32x4_t* s, int p, frag b, f32x4_t c) { return mfma(s[p], b, c); }
-    // column fragment x weights, as the second operand of the state's product
-    struct weighted { frag v; };
-    static __device__ __forceinline__ weighted weigh(frag v, const float* w) {
-        weighted t;
+    static __device__ __forceinline__ void of_state(const f32x4_t* s, int p, frag (&f)[1]) { f[0] = s[p]; }
+    static __device__ __forceinline__ void weigh(frag v, const float* w, frag (&f)[1], bool) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) t.v[r] = v[r] * w[r];
-        return t;
+        for (int r = 0; r < 4; ++r) f[0][r] = v[r] * w[r];
     }
-    static __device__ __forceinline__ f32x4_t mfma_weighted(frag a, const weighted& w, f32x4_t c) { return mfma(a, w.v, c); }
     static __device__ __forceinline__ void store_p(float* p, int plane, f32x4_t v) { (void)plane; *reinterpret_cast<f32x4_t*>(p) = v; }
-    static __device__ __forceinline__ f32x4_t mfma_p(frag c, const float* p, int plane, int q, int g, f32x4_t o) { (void)plane; return mfma(c, row(p, q, g), o); }
-    static __device__ __forceinline__ void store_out(float* o, f32x4_t v, bool vec, int left) {
-        if (vec) { if (left > 0) *reinterpret_cast<f32x4_t*>(o) = v; }
-        else
-#pragma unroll
-            for (int r = 0; r < 4; ++r) if (r < left) o[r] = v[r];
-    }
+    static __device__ __forceinline__ void store_out(float* o, f32x4_t v) { *reinterpret_cast<f32x4_any_t*>(o) = v; }
 };
 
 template <> struct mix_ops<bf16_t> {
-    static constexpr int KB = 32, PAD = 8, PLANES = 2;
+    static constexpr int KB = 32, PAD = 8, STEPS = 1, P_PARTS = 2, S_PARTS = 2, W_PARTS = 3;
     typedef u32x4_t frag;                                        // eight bf16
-    typedef unsigned short u16;
     static __device__ __forceinline__ u32x2_t two(const bf16_t* p) { return *reinterpret_cast<const u32x2_t*>(p); }
     // k = 32 p + 4 g + r and 32 p + 16 + 4 g + r: the order in which two state tiles hold their rows
     static __device__ __forceinline__ frag row(const bf16_t* r, int p, int g) {
@@ -93,7 +79,7 @@ template <> struct mix_ops<bf16_t> {
     }
     static __device__ __forceinline__ frag row_natural(const bf16_t* r, int p, int g) { return *reinterpret_cast<const u32x4_t*>(r + 32 * p + 8 * g); }
     // a column, rows 32 p + 8 g + 0..7, by the transposing LDS read (lane q of 16 names row q / 4, columns 4 (q % 4) and receives column q of
-    // four rows).  col: the first of the 16 columns.
+    // four rows)
     static __device__ __forceinline__ frag column(const bf16_t* base, int stride, int p, int g, int col) {
         const int q = threadIdx.x & 15;
         typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -104,36 +90,35 @@ template <> struct mix_ops<bf16_t> {
         const frag v = {x.x, x.y, y.x, y.y};
         return v;
     }
-    static __device__ __forceinline__ f32x4_t mfma(frag a, frag b, f32x4_t c) {
+    static __device__ __forceinline__ f32x4_t mfma(frag a, frag b, f32x4_t c, int) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
     }
     static __device__ __forceinline__ void split2(float x0, float x1, unsigned& h, unsigned& l) {
         h = cvt_pk_bf16(x0, x1);
         l = cvt_pk_bf16(x0 - __uint_as_float(h << 16), x1 - __uint_as_float(h & 0xffff0000u));
     }
-    static __device__ __forceinline__ f32x4_t mfma_state(const f32x4_t* s, int p, frag b, f32x4_t c) {
-        frag h, l;
+    static __device__ __forceinline__ void of_state(const f32x4_t* s, int p, frag (&f)[2]) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const f32x4_t t = s[2 * p + (q >> 1)];
             unsigned x, y;
             split2(t[2 * (q & 1)], t[2 * (q & 1) + 1], x, y);
-            h[q] = x; l[q] = y;
+            f[0][q] = x; f[1][q] = y;
         }
-        return mfma(h, b, mfma(l, b, c));
     }
-    struct weighted { frag h, m, l; };
-    static __device__ __forceinline__ weighted weigh(frag v, const float* w) {
-        weighted t;
+    // the third part where the state is a result
+    static __device__ __forceinline__ void weigh(frag v, const float* w, frag (&f)[3], bool third) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            unsigned x, y, z;
-            split3_pair(__uint_as_float(v[q] << 16) * w[2 * q], __uint_as_float(v[q] & 0xffff0000u) * w[2 * q + 1], x, y, z);
-            t.h[q] = x; t.m[q] = y; t.l[q] = z;
+            const float x = __uint_as_float(v[q] << 16) * w[2 * q], y = __uint_as_float(v[q] & 0xffff0000u) * w[2 * q + 1];
+            unsigned hi, lo;
+            split2(x, y, hi, lo);
+            f[0][q] = hi; f[1][q] = lo;
+            if (third)
+                f[2][q] = cvt_pk_bf16((x - __uint_as_float(hi << 16)) - __uint_as_float(lo << 16),
+                                      (y - __uint_as_float(hi & 0xffff0000u)) - __uint_as_float(lo & 0xffff0000u));
         }
-        return t;
     }
-    static __device__ __forceinline__ f32x4_t mfma_weighted(frag a, const weighted& w, f32x4_t c) { return mfma(a, w.h, mfma(a, w.m, mfma(a, w.l, c))); }
     static __device__ __forceinline__ void store_p(bf16_t* p, int plane, f32x4_t v) {
         unsigned h0, l0, h1, l1;
         split2(v[0], v[1], h0, l0);
@@ -142,54 +127,93 @@ template <> struct mix_ops<bf16_t> {
         *reinterpret_cast<u32x2_t*>(p) = h;
         *reinterpret_cast<u32x2_t*>(p + plane) = l;
     }
-    static __device__ __forceinline__ f32x4_t mfma_p(frag c, const bf16_t* p, int plane, int q, int g, f32x4_t o) {
-        return mfma(c, row_natural(p, q, g), mfma(c, row_natural(p + plane, q, g), o));
-    }
-    static __device__ __forceinline__ void store_out(bf16_t* o, f32x4_t v, bool vec, int left) {
-        if (vec) {
-            const u32x2_t t = {cvt_pk_bf16(v[0], v[1]), cvt_pk_bf16(v[2], v[3])};
-            if (left > 0) *reinterpret_cast<u32x2_t*>(o) = t;
-        } else
-#pragma unroll
-            for (int r = 0; r < 4; ++r) if (r < left) io_store(o + r, v[r]);
+    static __device__ __forceinline__ void store_out(bf16_t* o, f32x4_t v) {
+        typedef u32x2_t any_t __attribute__((aligned(2)));
+        *reinterpret_cast<any_t*>(o) = u32x2_t{cvt_pk_bf16(v[0], v[1]), cvt_pk_bf16(v[2], v[3])};
     }
 };
 
-// 64 rows of a tensor on their way from memory to LDS: N 16-byte pieces per thread, pieces of a row by neighbouring threads
-template <typename E, int D, int NT>
+// s elements off the low end of 16 bytes, 0 in at the high end
+template <typename E>
+__device__ __forceinline__ u32x4_t drop_low(u32x4_t v, int s) {
+    const int bits = s * 8 * (int)sizeof(E), words = bits >> 5, rest = bits & 31;
+    u32x4_t a;
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+        unsigned x = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (m + k < 4) x = words == k ? v[m + k] : x;
+        a[m] = x;
+    }
+    if (sizeof(E) == 2 && rest) {
+#pragma unroll
+        for (int m = 0; m < 4; ++m) a[m] = (a[m] >> 16) | (m < 3 ? a[m + 1] << 16 : 0u);
+    }
+    return a;
+}
+
+// 64 rows of a tensor on their way from memory to LDS: N 16-byte pieces per thread, pieces of a row by neighbouring threads.  Rows come in
+// the order of memory and are turned round in LDS for reversed time.  Requests are never conditional -- a load under a branch makes the
+// compiler wait for all loads wherever one is used -- but stay inside the tensor: rows behind the sequence are requested as its last one,
+// pieces behind the row's end from its last 16 bytes; store() puts that right.
+// FULL: d is D, and 64 rows span less than 2 GB: an address is a scalar base and a 32-bit offset that the thread keeps.
+template <typename E, int D, int NT, bool FULL>
 struct mix_stage_t {
-    static constexpr int PER = 16 / sizeof(E), ROW = D / PER, N = (CH * ROW + NT - 1) / NT, STRIDE = D + mix_ops<E>::PAD;
+    static constexpr int PER = 16 / sizeof(E), ROW = D / PER, N = (CH * ROW + NT - 1) / NT, STRIDE = D + mix_ops<E>::PAD, STEP = NT / ROW;
+    static constexpr bool ALL = N * NT == CH * ROW;             // else the threads left over request what is there already, and store nothing
     u32x4_t v[N];
-    // rows first .. first + 63 of n (in reversed time the rows counted from the end); absent rows and columns read as 0
-    __device__ __forceinline__ void load(const E* base, int64_t stride, int first, int n, int reverse, int d, bool vec, int tid) {
+    const E* base;
+    int64_t stride;
+    int d, n, reverse, row0, at0;                               // this thread's first row and its element of a row
+    unsigned off0;
+    __device__ __forceinline__ void begin(const E* base_, int64_t stride_, int d_, int n_, int reverse_, int tid) {
+        base = base_; stride = stride_; d = d_; n = n_; reverse = reverse_;
+        row0 = ALL ? tid / ROW : min(tid / ROW, CH - 1);
+        at0 = (tid % ROW) * PER;
+        off0 = FULL ? (unsigned)row0 * (unsigned)((int)stride * (int)sizeof(E)) + (unsigned)at0 * (unsigned)sizeof(E) : 0u;
+    }
+    // steps first .. first + 63 of n > first
+    __device__ __forceinline__ void load(int first) {
+        const int left = n - first, low = reverse ? left - CH : first;          // memory row of the chunk's first row (can be below 0)
+        const int row_min = reverse ? max(CH - left, 0) : 0, row_max = reverse ? CH - 1 : min(left, CH) - 1;
+        const char* at = reinterpret_cast<const char*>(base + (int64_t)low * stride);
+        if (FULL && left >= CH) {
 #pragma unroll
-        for (int q = 0; q < N; ++q) {
-            const int at = tid + q * NT, r = at / ROW, c = (at % ROW) * PER, i = first + r;
-            u32x4_t x = {0, 0, 0, 0};
-            if ((N * NT == CH * ROW || r < CH) && i < n && c < d) {
-                const E* row = base + (int64_t)(reverse ? n - 1 - i : i) * stride + c;
-                if (vec) x = *reinterpret_cast<const u32x4_t*>(row);
+            for (int q = 0; q < N; ++q) v[q] = row16<E>::load(reinterpret_cast<const E*>(at + (int64_t)(q * STEP) * stride * (int)sizeof(E) + off0));
+        } else {
+#pragma unroll
+            for (int q = 0; q < N; ++q) {
+                const E* row = reinterpret_cast<const E*>(at) + (int64_t)min(max(row0 + q * STEP, row_min), row_max) * stride;
+                if (FULL || d >= PER) v[q] = row16<E>::load(row + (FULL ? at0 : min(at0, d - PER)));
                 else {
-                    if (sizeof(E) == 4) {
 #pragma unroll
-                        for (int m = 0; m < 4; ++m) x[m] = c + m < d ? reinterpret_cast<const unsigned*>(row)[m] : 0u;
-                    } else {
-#pragma unroll
-                        for (int m = 0; m < 8; ++m) {
-                            const unsigned e = c + m < d ? reinterpret_cast<const unsigned short*>(row)[m] : 0u;
-                            x[m >> 1] |= e << (16 * (m & 1));
-                        }
-                    }
+                    for (int m = 0; m < PER; ++m) row16<E>::put(v[q], m, row16<E>::bits(row + min(at0 + m, d - 1)));
                 }
             }
-            v[q] = x;
         }
     }
-    __device__ __forceinline__ void store(E* lds, int tid) const {
+    __device__ __forceinline__ void store(E* lds, int left, int tid) {
+        if (!FULL || left < CH) {
 #pragma unroll
-        for (int q = 0; q < N; ++q) {
-            const int at = tid + q * NT, r = at / ROW, c = (at % ROW) * PER;
-            if (N * NT == CH * ROW || r < CH) *reinterpret_cast<u32x4_t*>(lds + r * STRIDE + c) = v[q];
+            for (int q = 0; q < N; ++q) {
+                const int row = row0 + q * STEP;
+                const u32x4_t zero = {0, 0, 0, 0};
+                if (!FULL) {
+                    if (d < PER) {
+#pragma unroll
+                        for (int m = 0; m < PER; ++m)
+                            if (at0 + m >= d) row16<E>::put(v[q], m, 0u);
+                    } else if (at0 + PER > d) v[q] = at0 < d ? drop_low<E>(v[q], at0 + PER - d) : zero;
+                }
+                if ((reverse ? CH - 1 - row : row) >= left) v[q] = zero;
+            }
+        }
+        if (ALL || tid < CH * ROW) {
+            E* to = lds + (reverse ? CH - 1 - row0 : row0) * STRIDE + at0;
+            const int step = reverse ? -STEP * STRIDE : STEP * STRIDE;
+#pragma unroll
+            for (int q = 0; q < N; ++q) *reinterpret_cast<u32x4_t*>(to + q * step) = v[q];
         }
     }
 };
@@ -197,193 +221,303 @@ struct mix_stage_t {
 template <typename E, int DA, int NW>
 struct mix_geom {
     static constexpr int DC = 16 * NW, NT = 64 * NW, SA = DA + mix_ops<E>::PAD, SC = DC + mix_ops<E>::PAD, SP = CH + mix_ops<E>::PAD;
-    static constexpr int A = 0, B = A + CH * SA, C = B + CH * SA, P = C + CH * SC, END = P + mix_ops<E>::PLANES * CH * SP;
+    static constexpr int A = 0, B = A + CH * SA, C = B + CH * SA, P = C + CH * SC, END = P + mix_ops<E>::P_PARTS * CH * SP;
     static constexpr int BYTES = END * (int)sizeof(E);
+    static constexpr int FIT = NW * (160 * 1024 / (BYTES + 2048)), MIN_WAVES = FIT >= 8 ? 2 : 1;      // waves of a compute unit, and so of a SIMD, that LDS has room for
 };
 
-template <typename E, int DA, int NW>
-__global__ void __launch_bounds__(64 * NW) linattn_mix_kernel(mix_t p) {
+template <typename E, int DA, int NW, bool FULL>
+__global__ void __launch_bounds__(64 * NW, (mix_geom<E, DA, NW>::MIN_WAVES)) linattn_mix_kernel(mix_t p) {
     typedef mix_ops<E> M;
     typedef mix_geom<E, DA, NW> G;
-    constexpr int NT = G::NT, NPA = DA / M::KB, NPC = CH / M::KB, TPP = M::KB / 16;      // fragments over DA, over a chunk; tiles per fragment
+    typedef typename M::frag frag;
+    constexpr int NT = G::NT, TILES = DA / 16, NPA = DA / M::KB, NPC = CH / M::KB, TPP = M::KB / 16;     // fragments over DA, over a chunk; tiles of one
+    constexpr int PLANE = CH * G::SP;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds_raw[];
     E* la = reinterpret_cast<E*>(lds_raw) + G::A;
     E* lb = reinterpret_cast<E*>(lds_raw) + G::B;
     E* lc = reinterpret_cast<E*>(lds_raw) + G::C;
     E* lp = reinterpret_cast<E*>(lds_raw) + G::P;
-    __shared__ float pw[CH + 1], wq[CH], wb[CH];
+    // powers of lam: 0..64 and that of the last chunk's steps; those of the scores by i - j + 16, 0 for i < j; weights of a S and of c by step, of
+    // whole chunks without a cut [0] and of the chunk at hand otherwise [1]
+    __shared__ float pw[CH + 2], pw_low[CH + 2], score_w[CH + 16], wq[2][CH], wb[2][CH];
     __shared__ int seg_of[CH];
     // workgroups of one row and head follow each other on one XCD (ids go round the 8 of them): its jobs share their reads in that L2
-    const int lin = blockIdx.x, turn = lin >> 3;
-    const int job_i = turn % p.n_jobs, unit = (turn / p.n_jobs) * 8 + (lin & 7);
+    const int lin = blockIdx.x, turn = lin >> 3, both = turn % (p.n_jobs * p.n_slices);
+    const int job_i = both / p.n_slices, unit = turn / (p.n_jobs * p.n_slices) * 8 + (lin & 7);
     if (unit >= p.B * p.H * p.n_seg) return;
     const mix_job_t& J = p.job[job_i];
     const int bh = unit / p.n_seg, seg = unit % p.n_seg, b = bh / p.H, h = bh % p.H;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), ln = lane & 15, g = lane >> 4;
     const int n = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
     const int c_first = seg * p.seg_chunks, c_end = min(c_first + p.seg_chunks, (n + CH - 1) / CH);
-    const int da = J.da, dc = J.dc;
-    const E* pa = (const E*)J.a + b * J.sa[1] + h * J.sa[2];
-    const E* pb = (const E*)J.b + b * J.sb[1] + h * J.sb[2];
-    const E* pc = (const E*)J.c + b * J.sc[1] + h * J.sc[2];
-    E* po = (E*)J.out + b * J.so[1] + h * J.so[2];
-    float gl = p.log_decay[h];
-    gl = gl > 0.f ? 0.f : gl < -1e30f ? -1e30f : gl;
-    if (tid <= CH) pw[tid] = (float)exp((double)gl * tid);
-    if (NT == 64 && tid == 0) pw[CH] = (float)exp((double)gl * CH);
-    const int n_last = n - (n - 1) / CH * CH;                       // steps of the row's last chunk (n > 0)
-    const double full = exp((double)gl * CH), part = exp((double)gl * n_last);
-    const float full_h = (float)full, full_l = (float)(full - (double)full_h), part_h = (float)part, part_l = (float)(part - (double)part_h);
+    const int c0 = (both % p.n_slices) * G::DC;                     // the slice of c's columns
+    const int da = FULL ? DA : J.da, dc = FULL ? G::DC : min(J.dc - c0, G::DC), reverse = J.reverse, off = J.off;
+    if (!FULL && dc <= 0) return;                                   // a job of fewer columns than the widest
+    const bool states_only = p.states_only;
+    const float scale_p = J.scale_p, scale_s = J.scale_s, scale_b = J.scale_b;
+    const float* reset = p.reset;
+    E* po = (E*)J.out + b * J.so[1] + h * J.so[2] + c0;
+    const int64_t so = J.so[0];
 
-    f32x4_t S[DA / 16];
-    {
-        const float* s = J.s_in ? J.s_in + ((int64_t)bh * p.n_seg + seg) * J.s_row : nullptr;
-        const int e = 16 * w + ln;
-#pragma unroll
-        for (int t = 0; t < DA / 16; ++t)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int d = 16 * t + 4 * g + r;
-                S[t][r] = (s && d < da && e < dc) ? s[d * J.sd + e * J.se] : 0.f;
-            }
-    }
-    if (!p.states_only) {
-        // P's tiles above the diagonal that share a fragment with one on it are read and stay 0
-        if (TPP == 2)
-            for (int at = tid; at < 2 * 32 * M::PLANES; at += NT) {
-                const int plane = at / 64, r = at % 64, i = (r >> 4) * 32 + (r & 15);      // rows 0..15 and 32..47
-                if (r < 32) {
-                    u32x4_t* z = reinterpret_cast<u32x4_t*>(lp + plane * CH * G::SP + i * G::SP + (i & 32) + 16);
-                    const u32x4_t zero = {0, 0, 0, 0};
-                    z[0] = zero; z[1] = zero;
-                }
-            }
-        // rows behind the sequence: 0
-        const int lo = max(n, c_first * CH), hi = min(p.T, (c_first + p.seg_chunks) * CH);
-        for (int64_t at = (int64_t)lo * dc + tid; at < (int64_t)hi * dc; at += NT) io_store(po + (at / dc) * J.so[0] + at % dc, 0.f);
-    }
-
-    // weights of the scores: lam^(16 dist + ln - (4 g + r)), masked above the diagonal, for the four distances of two tiles
-    lds_barrier();
-    float wd[4][4];
-#pragma unroll
-    for (int dist = 0; dist < 4; ++dist)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int k = 16 * dist + ln - 4 * g - r;
-            wd[dist][r] = k >= 0 ? J.scale_p * pw[k] : 0.f;
-        }
-
-    mix_stage_t<E, DA, NT> ra, rb;
-    mix_stage_t<E, G::DC, NT> rc;
+    mix_stage_t<E, DA, NT, FULL> ra, rb;
+    mix_stage_t<E, G::DC, NT, FULL> rc;
+    ra.begin((const E*)J.a + b * J.sa[1] + h * J.sa[2], J.sa[0], da, n, reverse, tid);
+    rb.begin((const E*)J.b + b * J.sb[1] + h * J.sb[2], J.sb[0], da, n, reverse, tid);
+    rc.begin((const E*)J.c + b * J.sc[1] + h * J.sc[2] + c0, J.sc[0], dc, n, reverse, tid);
     float rflag = 0.f;
     auto request = [&](int c) {
         const int first = c * CH;
-        if (!p.states_only) ra.load(pa, J.sa[0], first, n, J.reverse, da, J.vec & 1, tid);
-        rb.load(pb, J.sb[0], first, n, J.reverse, da, J.vec & 2, tid);
-        rc.load(pc, J.sc[0], first, n, J.reverse, dc, J.vec & 4, tid);
-        if (p.reset) {
+        if (!states_only) ra.load(first);
+        rb.load(first);
+        rc.load(first);
+        if (reset) {
             // what came before step i is cut off: by the reset of step i; in reversed time by that of the step behind it
-            const int i = first + lane, t = J.reverse ? n - i : i;
-            rflag = (i < n && t < n) ? p.reset[(int64_t)t * p.B + b] : 0.f;
+            const int i = first + lane, t = reverse ? n - i : i;
+            rflag = reset[(int64_t)min(max(t, 0), n - 1) * p.B + b];           // of another step where there is none: see below
         }
     };
-    bool cut_any = false;
     if (c_first < c_end) request(c_first);
+
+    float gl = p.log_decay[h];
+    gl = gl > 0.f ? 0.f : gl < -1e30f ? -1e30f : gl;
+    const int n_last = n - (n - 1) / CH * CH;                       // steps of the row's last chunk (n > 0)
+    for (int k = tid; k < CH + 2; k += NT) {
+        const double f = exp((double)gl * (k <= CH ? k : n_last));
+        pw[k] = (float)f;
+        pw_low[k] = (float)(f - (double)(float)f);
+    }
+    f32x4_t S[TILES];
+    {
+        const float* s = J.s_in;
+        const int e = 16 * w + ln;
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) S[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        if (s) {
+            s += ((int64_t)bh * p.n_seg + seg) * J.s_row + (c0 + e) * J.se;
+            const int sd = J.sd;
+#pragma unroll
+            for (int t = 0; t < TILES; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int d = 16 * t + 4 * g + r;
+                    if (FULL || (d < da && e < dc)) S[t][r] = s[d * sd];
+                }
+        }
+    }
+    const bool fine = states_only || (J.s_out && p.n_seg == 1);      // the state is a result
+    if (!states_only) {
+        // P's tiles above the diagonal that share a fragment with one on it are read and stay 0
+        if (TPP == 2)
+            for (int at = tid; at < 32 * M::P_PARTS; at += NT) {
+                const int i = ((at >> 4) & 1) * 32 + (at & 15);                           // rows 0..15 and 32..47
+                u32x4_t* z = reinterpret_cast<u32x4_t*>(lp + (at >> 5) * PLANE + i * G::SP + (i & 32) + 16);
+                const u32x4_t zero = {0, 0, 0, 0};
+                z[0] = zero; z[1] = zero;
+            }
+        // rows behind the sequence: 0
+        const int lo = max(n, c_first * CH), hi = min(p.T, (c_first + p.seg_chunks) * CH);
+        constexpr int PIECES = G::DC / 4;
+        for (int r = lo + tid / PIECES; r < hi; r += NT / PIECES) {
+            const int e = tid % PIECES * 4;
+            E* o = po + (int64_t)r * so + e;
+            if (e + 4 <= dc) M::store_out(o, f32x4_t{0.f, 0.f, 0.f, 0.f});
+            else
+                for (int m = 0; e + m < dc; ++m) io_store(o + m, 0.f);
+        }
+    }
+    lds_barrier();
+    for (int k = tid; k < CH + 16; k += NT) score_w[k] = k < 16 ? 0.f : scale_p * pw[max(k - 16, 0)];
+    if (tid < CH) {
+        wq[0][tid] = scale_s * pw[tid + off];
+        wb[0][tid] = scale_b * pw[CH - tid - off];
+    }
+
+    bool cut_any = false;
     for (int c = c_first; c < c_end; ++c) {
-        const int nv = min(CH, n - c * CH);
+        const int left = n - c * CH;
         unsigned long long cuts = 0;
-        if (p.reset) cuts = __ballot(rflag != 0.f);
+        if (reset) {
+            const int i = c * CH + lane;
+            cuts = __ballot(rflag != 0.f && i < n && (!reverse || i > 0));
+        }
         cut_any = cut_any || cuts != 0;
-        if (!p.states_only) ra.store(la, tid);
-        rb.store(lb, tid);
-        rc.store(lc, tid);
-        const int n_cuts = __popcll(cuts);
-        if (tid < CH) {
-            const int k = __popcll(cuts & (~0ull >> (63 - tid)));      // cuts up to and including this step
+        if (!states_only) ra.store(la, left, tid);
+        rb.store(lb, left, tid);
+        rc.store(lc, left, tid);
+        const int own_w = cuts != 0 || left < CH ? 1 : 0;
+        if (own_w && tid < CH) {
+            const int nv = min(left, CH), k = __popcll(cuts & (~0ull >> (63 - tid)));      // cuts up to and including this step
+            const float q = pw[tid + off], x = pw[max(nv - tid - off, 0)];
             seg_of[tid] = k;
-            wq[tid] = k == 0 ? J.scale_s * pw[tid + J.off] : 0.f;
-            wb[tid] = (tid < nv && k == n_cuts) ? J.scale_b * pw[nv - tid - J.off] : 0.f;
+            wq[1][tid] = k == 0 ? scale_s * q : 0.f;
+            wb[1][tid] = tid < nv && k == __popcll(cuts) ? scale_b * x : 0.f;
         }
         lds_barrier();
         if (c + 1 < c_end) request(c + 1);
         f32x4_t O[4];
-        if (!p.states_only) {
-            // P^T tiles on and below the diagonal, dealt out to the waves
-            for (int t = w; t < 10; t += NW) {
-                const int it = t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3, jt = t - it * (it + 1) / 2;
-                f32x4_t s = {0.f, 0.f, 0.f, 0.f};
+        if (!states_only) {
+            // P^T tiles on and below the diagonal, dealt out to the waves, up to three at a time
+            constexpr int MINE = (10 + NW - 1) / NW, AT_ONCE = MINE < 3 ? MINE : 3;
 #pragma unroll
-                for (int q = 0; q < NPA; ++q) s = M::mfma(M::row(lb + (16 * jt + ln) * G::SA, q, g), M::row(la + (16 * it + ln) * G::SA, q, g), s);
-                const int dist = it - jt;
+            for (int t0 = 0; t0 < MINE; t0 += AT_ONCE) {
+                f32x4_t s[AT_ONCE];
+                int it[AT_ONCE], jt[AT_ONCE];
+                const E *ax[AT_ONCE], *bx[AT_ONCE];
+                float sw[AT_ONCE][4];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) s[r] *= dist == 0 ? wd[0][r] : dist == 1 ? wd[1][r] : dist == 2 ? wd[2][r] : wd[3][r];
-                if (cuts) {
-                    const int k = seg_of[16 * it + ln];
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) s[r] = seg_of[16 * jt + 4 * g + r] == k ? s[r] : 0.f;
+                for (int k = 0; k < AT_ONCE; ++k) {
+                    const int t = min(w + (t0 + k) * NW, 9);                          // a wave without one repeats the last: the same values again
+                    it[k] = t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3;
+                    jt[k] = t - it[k] * (it[k] + 1) / 2;
+                    s[k] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+                    ax[k] = la + (16 * it[k] + ln) * G::SA;
+                    bx[k] = lb + (16 * jt[k] + ln) * G::SA;
                 }
-                M::store_p(lp + (16 * it + ln) * G::SP + 16 * jt + 4 * g, CH * G::SP, s);
+                frag fa[2][AT_ONCE], fb[2][AT_ONCE];
+#pragma unroll
+                for (int q = 0; q <= NPA; ++q) {                                      // one fragment ahead of the matrix instructions
+                    if (q < NPA) {
+#pragma unroll
+                        for (int k = 0; k < AT_ONCE; ++k) { fb[q & 1][k] = M::row(bx[k], q, g); fa[q & 1][k] = M::row(ax[k], q, g); }
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < AT_ONCE; ++k)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) sw[k][r] = score_w[16 + 16 * (it[k] - jt[k]) + ln - 4 * g - r];
+                    }
+                    if (q > 0) {
+#pragma unroll
+                        for (int x = 0; x < M::STEPS; ++x)
+#pragma unroll
+                            for (int k = 0; k < AT_ONCE; ++k)
+                                if (t0 + k < MINE) s[k] = M::mfma(fb[(q - 1) & 1][k], fa[(q - 1) & 1][k], s[k], x);
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < AT_ONCE; ++k)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[k][r] *= sw[k][r];
+                if (cuts) {
+#pragma unroll
+                    for (int k = 0; k < AT_ONCE; ++k) {
+                        const int m = seg_of[16 * it[k] + ln];
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) s[k][r] = seg_of[16 * jt[k] + 4 * g + r] == m ? s[k][r] : 0.f;
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < AT_ONCE; ++k)
+                    if (t0 + k < MINE) M::store_p(lp + (16 * it[k] + ln) * G::SP + 16 * jt[k] + 4 * g, PLANE, s[k]);
             }
 #pragma unroll
-            for (int it = 0; it < 4; ++it) {
-                f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+            for (int it = 0; it < 4; ++it) O[it] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+            frag fa[2][4];
+            float fq[4];
 #pragma unroll
-                for (int q = 0; q < NPA; ++q) o = M::mfma_state(S, q, M::row(la + (16 * it + ln) * G::SA, q, g), o);
-                const float f = wq[16 * it + ln];
+            for (int q = 0; q <= NPA; ++q) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) o[r] *= f;
-                O[it] = o;
+                for (int it = 0; it < 4; ++it) {
+                    if (q < NPA) fa[q & 1][it] = M::row(la + (16 * it + ln) * G::SA, q, g);
+                    else fq[it] = wq[own_w][16 * it + ln];
+                }
+                if (q > 0) {
+                    frag fs[M::S_PARTS];
+                    M::of_state(S, q - 1, fs);
+#pragma unroll
+                    for (int part = M::S_PARTS - 1; part >= 0; --part)
+#pragma unroll
+                        for (int x = 0; x < M::STEPS; ++x)
+#pragma unroll
+                            for (int it = 0; it < 4; ++it) O[it] = M::mfma(fs[part], fa[(q - 1) & 1][it], O[it], x);
+                }
             }
+#pragma unroll
+            for (int it = 0; it < 4; ++it)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) O[it][r] *= fq[it];
             lds_barrier();
         }
         {
-            const bool last = nv < CH || (c + 1) * CH == n;
-            float ch = full_h, cl = full_l;
-            if (last) { ch = part_h; cl = part_l; }
-            if (cuts) ch = cl = 0.f;
+            const bool last = left <= CH;
+            const float ch = cuts ? 0.f : pw[last ? CH + 1 : CH], cl = cuts ? 0.f : pw_low[last ? CH + 1 : CH];
+            // where half of the state or more is gone a chunk later, the rounding of lam^64 does not add up over the chunks
+            if (__builtin_amdgcn_readfirstlane(ch > 0.5f)) {
 #pragma unroll
-            for (int t = 0; t < DA / 16; ++t)
+                for (int t = 0; t < TILES; ++t)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) S[t][r] = __builtin_fmaf(S[t][r], ch, S[t][r] * cl);
+                    for (int r = 0; r < 4; ++r) S[t][r] = __builtin_fmaf(S[t][r], ch, S[t][r] * cl);
+            } else {
+#pragma unroll
+                for (int t = 0; t < TILES; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) S[t][r] *= ch;
+            }
         }
 #pragma unroll
         for (int q = 0; q < NPC; ++q) {
-            const typename M::frag cf = M::column(lc, G::SC, q, g, 16 * w + ln);
-            if (!p.states_only) {
-#pragma unroll
-                for (int it = 0; it < 4; ++it)
-                    if (q * TPP <= it) O[it] = M::mfma_p(cf, lp + (16 * it + ln) * G::SP, CH * G::SP, q, g, O[it]);
-            }
+            const frag cf = M::column(lc, G::SC, q, g, 16 * w + ln);
+            frag cw[M::W_PARTS], fp[M::P_PARTS][4], fb[TILES];
             float wv[M::KB / 4];
 #pragma unroll
-            for (int r = 0; r < M::KB / 4; ++r) wv[r] = wb[M::KB * q + (M::KB / 4) * g + r];
-            const typename M::weighted cw = M::weigh(cf, wv);
+            for (int r = 0; r < M::KB / 4; ++r) wv[r] = wb[own_w][M::KB * q + (M::KB / 4) * g + r];
+            if (!states_only) {
 #pragma unroll
-            for (int t = 0; t < DA / 16; ++t) S[t] = M::mfma_weighted(M::column(lb, G::SA, q, g, 16 * t + ln), cw, S[t]);
+                for (int part = 0; part < M::P_PARTS; ++part)
+#pragma unroll
+                    for (int it = 0; it < 4; ++it)
+                        if (q * TPP <= it) fp[part][it] = M::row_natural(lp + part * PLANE + (16 * it + ln) * G::SP, q, g);
+            }
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) fb[t] = M::column(lb, G::SA, q, g, 16 * t + ln);
+            if (!states_only) {
+#pragma unroll
+                for (int part = M::P_PARTS - 1; part >= 0; --part)
+#pragma unroll
+                    for (int x = 0; x < M::STEPS; ++x)
+#pragma unroll
+                        for (int it = 0; it < 4; ++it)
+                            if (q * TPP <= it) O[it] = M::mfma(cf, fp[part][it], O[it], x);
+            }
+            M::weigh(cf, wv, cw, fine);
+#pragma unroll
+            for (int part = M::W_PARTS - 1; part >= 0; --part) {
+                if (part == 2 && !fine) continue;
+#pragma unroll
+                for (int x = 0; x < M::STEPS; ++x)
+#pragma unroll
+                    for (int t = 0; t < TILES; ++t) S[t] = M::mfma(fb[t], cw[part], S[t], x);
+            }
         }
-        if (!p.states_only) {
-            const int e = 16 * w + 4 * g;
+        if (!states_only) {
+            // rows of O in the order of memory, as the stage's
+            const int low = reverse ? left - CH : c * CH, e = 16 * w + 4 * g;
+            E* at = po + (int64_t)low * so + (int64_t)(reverse ? 15 - ln : ln) * so + e;
 #pragma unroll
             for (int it = 0; it < 4; ++it) {
-                const int i = c * CH + 16 * it + ln;
-                if (i < n) M::store_out(po + (int64_t)(J.reverse ? n - 1 - i : i) * J.so[0] + e, O[it], J.vec & 8, dc - e);
+                E* o = at + (int64_t)(16 * (reverse ? 3 - it : it)) * so;
+                if (16 * it + ln < left) {
+                    if (FULL || e + 4 <= dc) M::store_out(o, O[it]);
+                    else
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) if (e + r < dc) io_store(o + r, O[it][r]);
+                }
             }
         }
         lds_barrier();
     }
     const int e = 16 * w + ln;
-    if (p.states_only) {
+    if (states_only) {
         const int64_t at = ((int64_t)bh * p.n_seg + seg);
-        float* s = J.s_out + at * J.da * J.dc;
+        float* s = J.s_out + at * p.kv + c0;
 #pragma unroll
         for (int t = 0; t < DA / 16; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int d = 16 * t + 4 * g + r;
-                if (d < da && e < dc) s[d * dc + e] = S[t][r];
+                if (d < da && e < dc) s[d * J.dc + e] = S[t][r];
             }
-        if (tid == 0) {
+        if (tid == 0 && c0 == 0) {
             const int steps = max(0, min(n, (c_first + p.seg_chunks) * CH) - c_first * CH);
             const double f = exp((double)gl * steps);
             J.carry[2 * at] = cut_any ? 0.f : (float)f;
@@ -396,60 +530,41 @@ __global__ void __launch_bounds__(64 * NW) linattn_mix_kernel(mix_t p) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int d = 16 * t + 4 * g + r;
-                if (d < da && e < dc) J.s_out[(int64_t)bh * p.kv + (int64_t)d * J.sd + (int64_t)e * J.se] = none ? 0.f : S[t][r];
+                if (d < da && e < dc) J.s_out[(int64_t)bh * p.kv + d * J.sd + (c0 + e) * J.se] = none ? 0.f : S[t][r];
             }
     }
 }
 
-template <typename E, int DA, int NW>
-static int launch_mix_as(const mix_t& m, hipStream_t s) {
+template <typename E, int DA, int NW, bool FULL>
+static int launch_mix_as(mix_t m, int dc, hipStream_t s) {
     typedef mix_geom<E, DA, NW> G;
-    static_assert(G::BYTES + 1200 <= 160 * 1024, "LDS");
-    const int64_t units = ((int64_t)m.B * m.H * m.n_seg + 7) / 8 * 8;
-    hipLaunchKernelGGL((linattn_mix_kernel<E, DA, NW>), dim3((unsigned)(units * m.n_jobs)), dim3(64 * NW), G::BYTES, s, m);
+    static_assert(G::BYTES + 1500 <= 160 * 1024, "LDS");
+    m.n_slices = (dc + G::DC - 1) / G::DC;
+    const int64_t units = ((int64_t)m.B * m.H * m.n_seg + 7) / 8 * 8, grid = units * m.n_jobs * m.n_slices;
+    XRL_CHECK_ARG(grid <= 0x7fffffff);
+    hipLaunchKernelGGL((linattn_mix_kernel<E, DA, NW, FULL>), dim3((unsigned)grid), dim3(64 * NW), G::BYTES, s, m);
     XRL_CHECK_LAUNCH();
     return XRL_OK;
 }
 
 template <typename E, int DA, int NW>
+static int launch_mix_size(const mix_t& m, int dc, hipStream_t s) {
+    bool full = true;
+    for (int i = 0; i < m.n_jobs; ++i) {
+        const mix_job_t& j = m.job[i];
+        full = full && j.da == DA && j.dc == dc && dc % (16 * NW) == 0;
+        const int64_t most = (1ll << 31) / (CH * (int)sizeof(E));
+        full = full && j.sa[0] < most && j.sb[0] < most && j.sc[0] < most;
+    }
+    return full ? launch_mix_as<E, DA, NW, true>(m, dc, s) : launch_mix_as<E, DA, NW, false>(m, dc, s);
+}
+
+template <typename E, int DA, int NW>
 static int init_mix_as() {
-    XRL_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(linattn_mix_kernel<E, DA, NW>), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                      mix_geom<E, DA, NW>::BYTES));
+    const int bytes = mix_geom<E, DA, NW>::BYTES;
+    XRL_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(linattn_mix_kernel<E, DA, NW, true>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    XRL_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(linattn_mix_kernel<E, DA, NW, false>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
     return XRL_OK;
-}
-
-// the instances that take more than 64 KB of LDS
-template <typename E>
-static int init_mix() {
-    if (int rc = init_mix_as<E, 64, 4>()) return rc;
-    if (int rc = init_mix_as<E, 64, 8>()) return rc;
-    if (int rc = init_mix_as<E, 128, 4>()) return rc;
-    return init_mix_as<E, 128, 8>();
-}
-
-// da, dc: the largest of the jobs'
-template <typename E>
-static int launch_mix(const mix_t& m, int da, int dc, hipStream_t s) {
-    const int nw = dc <= 16 ? 1 : dc <= 32 ? 2 : dc <= 64 ? 4 : 8;
-    if (sizeof(E) == 4 && da <= 16) {
-        if (nw == 1) return launch_mix_as<E, sizeof(E) == 4 ? 16 : 32, 1>(m, s);
-        if (nw == 2) return launch_mix_as<E, sizeof(E) == 4 ? 16 : 32, 2>(m, s);
-        if (nw == 4) return launch_mix_as<E, sizeof(E) == 4 ? 16 : 32, 4>(m, s);
-        return launch_mix_as<E, sizeof(E) == 4 ? 16 : 32, 8>(m, s);
-    }
-    if (da <= 32) {
-        if (nw == 1) return launch_mix_as<E, 32, 1>(m, s);
-        if (nw == 2) return launch_mix_as<E, 32, 2>(m, s);
-        if (nw == 4) return launch_mix_as<E, 32, 4>(m, s);
-        return launch_mix_as<E, 32, 8>(m, s);
-    }
-    if (da <= 64) {
-        if (nw <= 2) return launch_mix_as<E, 64, 2>(m, s);
-        if (nw == 4) return launch_mix_as<E, 64, 4>(m, s);
-        return launch_mix_as<E, 64, 8>(m, s);
-    }
-    if (nw <= 4) return launch_mix_as<E, 128, 4>(m, s);
-    return launch_mix_as<E, 128, 8>(m, s);
 }
 
 int launch_mix_f32(const mix_t& m, int da, int dc, hipStream_t s);
