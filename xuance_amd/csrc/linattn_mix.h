@@ -39,13 +39,14 @@ struct mix_t {
 
 constexpr int CH = 64;                    // steps of a chunk
 
-template <typename E> struct mix_ops;
+template <typename E, int TS> struct mix_ops;
 
 // Operands by fragments: KB values of k of 16 rows or columns.  A product of fragments takes STEPS matrix instructions; an f32 operand that is made
 // here (P, the state, the weighted c) takes P_PARTS, S_PARTS, W_PARTS fragments.
-template <> struct mix_ops<float> {
-    static constexpr int KB = 16, PAD = 4, STEPS = 4, P_PARTS = 1, S_PARTS = 1, W_PARTS = 1;
+template <> struct mix_ops<float, 16> {
+    static constexpr int KB = 16, PAD = 4, SLOTS = 4, STEPS = 4, P_PARTS = 1, S_PARTS = 1, W_PARTS = 1;
     typedef f32x4_t frag;
+    typedef f32x4_t acc;
     // four values of a row of LDS, k = 16 p + 4 g + r
     static __device__ __forceinline__ frag row(const float* r, int p, int g) { return *reinterpret_cast<const f32x4_t*>(r + 16 * p + 4 * g); }
     static __device__ __forceinline__ frag row_natural(const float* r, int p, int g) { return row(r, p, g); }
@@ -55,10 +56,8 @@ template <> struct mix_ops<float> {
         const f32x4_t v = {at[0], at[stride], at[2 * stride], at[3 * stride]};
         return v;
     }
-    static __device__ __forceinline__ f32x4_t mfma(frag a, frag b, f32x4_t c, int step) {
-        return __builtin_amdgcn_mfma_f32_16x16x4f32(a[step], b[step], c, 0, 0, 0);
-    }
-    static __device__ __forceinline__ void of_state(const f32x4_t* s, int p, frag (&f)[1]) { f[0] = s[p]; }
+    static __device__ __forceinline__ acc mfma(frag a, frag b, acc c, int step) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a[step], b[step], c, 0, 0, 0); }
+    static __device__ __forceinline__ void of_state(const acc* s, int p, frag (&f)[1]) { f[0] = s[p]; }
     static __device__ __forceinline__ void weigh(frag v, const float* w, frag (&f)[1], bool) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) f[0][r] = v[r] * w[r];
@@ -67,44 +66,24 @@ template <> struct mix_ops<float> {
     static __device__ __forceinline__ void store_out(float* o, f32x4_t v) { *reinterpret_cast<f32x4_any_t*>(o) = v; }
 };
 
-template <> struct mix_ops<bf16_t> {
-    static constexpr int KB = 32, PAD = 8, STEPS = 1, P_PARTS = 2, S_PARTS = 2, W_PARTS = 3;
+// what both tile sizes of bf16 share
+struct mix_bf16 {
+    static constexpr int PAD = 8, SLOTS = 8, STEPS = 1, P_PARTS = 2, S_PARTS = 2, W_PARTS = 3;
     typedef u32x4_t frag;                                        // eight bf16
     static __device__ __forceinline__ u32x2_t two(const bf16_t* p) { return *reinterpret_cast<const u32x2_t*>(p); }
-    // k = 32 p + 4 g + r and 32 p + 16 + 4 g + r: the order in which two state tiles hold their rows
-    static __device__ __forceinline__ frag row(const bf16_t* r, int p, int g) {
-        const u32x2_t x = two(r + 32 * p + 4 * g), y = two(r + 32 * p + 16 + 4 * g);
-        const frag v = {x.x, x.y, y.x, y.y};
-        return v;
-    }
-    static __device__ __forceinline__ frag row_natural(const bf16_t* r, int p, int g) { return *reinterpret_cast<const u32x4_t*>(r + 32 * p + 8 * g); }
-    // a column, rows 32 p + 8 g + 0..7, by the transposing LDS read (lane q of 16 names row q / 4, columns 4 (q % 4) and receives column q of
-    // four rows)
-    static __device__ __forceinline__ frag column(const bf16_t* base, int stride, int p, int g, int col) {
+    static __device__ __forceinline__ frag join(u32x2_t x, u32x2_t y) { return frag{x.x, x.y, y.x, y.y}; }
+    // eight rows of a column by two transposing LDS reads: lane q of 16 names row q / 4, columns 4 (q % 4) and receives column q of four rows
+    static __device__ __forceinline__ frag column16(const bf16_t* first, int stride) {
         const int q = threadIdx.x & 15;
         typedef short s16x4 __attribute__((ext_vector_type(4)));
         typedef __attribute__((address_space(3))) s16x4* lptr;
-        const bf16_t* at = base + (32 * p + 8 * g + (q >> 2)) * stride + (col - q) + 4 * (q & 3);
-        const u32x2_t x = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)at));
-        const u32x2_t y = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)(at + 4 * stride)));
-        const frag v = {x.x, x.y, y.x, y.y};
-        return v;
-    }
-    static __device__ __forceinline__ f32x4_t mfma(frag a, frag b, f32x4_t c, int) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+        const bf16_t* at = first + (q >> 2) * stride + 4 * (q & 3);
+        return join(__builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)at)),
+                    __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)(at + 4 * stride))));
     }
     static __device__ __forceinline__ void split2(float x0, float x1, unsigned& h, unsigned& l) {
         h = cvt_pk_bf16(x0, x1);
         l = cvt_pk_bf16(x0 - __uint_as_float(h << 16), x1 - __uint_as_float(h & 0xffff0000u));
-    }
-    static __device__ __forceinline__ void of_state(const f32x4_t* s, int p, frag (&f)[2]) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const f32x4_t t = s[2 * p + (q >> 1)];
-            unsigned x, y;
-            split2(t[2 * (q & 1)], t[2 * (q & 1) + 1], x, y);
-            f[0][q] = x; f[1][q] = y;
-        }
     }
     // the third part where the state is a result
     static __device__ __forceinline__ void weigh(frag v, const float* w, frag (&f)[3], bool third) {
@@ -133,6 +112,52 @@ template <> struct mix_ops<bf16_t> {
     }
 };
 
+template <> struct mix_ops<bf16_t, 16> : mix_bf16 {
+    static constexpr int KB = 32;
+    typedef f32x4_t acc;
+    // k = 32 p + 4 g + r and 32 p + 16 + 4 g + r: the order in which two state tiles hold their rows
+    static __device__ __forceinline__ frag row(const bf16_t* r, int p, int g) { return join(two(r + 32 * p + 4 * g), two(r + 32 * p + 16 + 4 * g)); }
+    static __device__ __forceinline__ frag row_natural(const bf16_t* r, int p, int g) { return *reinterpret_cast<const u32x4_t*>(r + 32 * p + 8 * g); }
+    static __device__ __forceinline__ frag column(const bf16_t* base, int stride, int p, int g, int col) {
+        return column16(base + (32 * p + 8 * g) * stride + (col & ~15), stride);
+    }
+    static __device__ __forceinline__ acc mfma(frag a, frag b, acc c, int) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ void of_state(const acc* s, int p, frag (&f)[2]) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const acc t = s[2 * p + (q >> 1)];
+            unsigned x, y;
+            split2(t[2 * (q & 1)], t[2 * (q & 1) + 1], x, y);
+            f[0][q] = x; f[1][q] = y;
+        }
+    }
+};
+
+// tiles of 32: half the LDS reads for the same products, twice the accumulators
+template <> struct mix_ops<bf16_t, 32> : mix_bf16 {
+    static constexpr int KB = 16;
+    typedef f32x16_t acc;
+    // k = 16 p + 4 g + r and 16 p + 8 + 4 g + r: the order in which half a state tile holds its rows
+    static __device__ __forceinline__ frag row(const bf16_t* r, int p, int g) { return join(two(r + 16 * p + 4 * g), two(r + 16 * p + 8 + 4 * g)); }
+    static __device__ __forceinline__ frag row_natural(const bf16_t* r, int p, int g) { return *reinterpret_cast<const u32x4_t*>(r + 16 * p + 8 * g); }
+    static __device__ __forceinline__ frag column(const bf16_t* base, int stride, int p, int g, int col) {
+        return column16(base + (16 * p + 8 * g) * stride + (col & ~15), stride);
+    }
+    static __device__ __forceinline__ acc mfma(frag a, frag b, acc c, int) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ void of_state(const acc* s, int p, frag (&f)[2]) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            unsigned x, y;
+            split2(s[p >> 1][8 * (p & 1) + 2 * q], s[p >> 1][8 * (p & 1) + 2 * q + 1], x, y);
+            f[0][q] = x; f[1][q] = y;
+        }
+    }
+};
+
 // s elements off the low end of 16 bytes, 0 in at the high end
 template <typename E>
 __device__ __forceinline__ u32x4_t drop_low(u32x4_t v, int s) {
@@ -158,27 +183,28 @@ __device__ __forceinline__ u32x4_t drop_low(u32x4_t v, int s) {
 // compiler wait for all loads wherever one is used -- but stay inside the tensor: rows behind the sequence are requested as its last one,
 // pieces behind the row's end from its last 16 bytes; store() puts that right.
 // FULL: d is D, and 64 rows span less than 2 GB: an address is a scalar base and a 32-bit offset that the thread keeps.
-template <typename E, int D, int NT, bool FULL>
+template <typename E, int D, int NT, bool FULL, int PAD>
 struct mix_stage_t {
-    static constexpr int PER = 16 / sizeof(E), ROW = D / PER, N = (CH * ROW + NT - 1) / NT, STRIDE = D + mix_ops<E>::PAD, STEP = NT / ROW;
+    static constexpr int PER = 16 / sizeof(E), ROW = D / PER, N = (CH * ROW + NT - 1) / NT, STRIDE = D + PAD, STEP = NT / ROW;
     static constexpr bool ALL = N * NT == CH * ROW;             // else the threads left over request what is there already, and store nothing
     u32x4_t v[N];
     const E* base;
     int64_t stride;
-    int d, n, reverse, row0, at0;                               // this thread's first row and its element of a row
-    unsigned off0;
-    __device__ __forceinline__ void begin(const E* base_, int64_t stride_, int d_, int n_, int reverse_, int tid) {
+    int d, n, reverse;
+    __device__ __forceinline__ void begin(const E* base_, int64_t stride_, int d_, int n_, int reverse_) {
         base = base_; stride = stride_; d = d_; n = n_; reverse = reverse_;
-        row0 = ALL ? tid / ROW : min(tid / ROW, CH - 1);
-        at0 = (tid % ROW) * PER;
-        off0 = FULL ? (unsigned)row0 * (unsigned)((int)stride * (int)sizeof(E)) + (unsigned)at0 * (unsigned)sizeof(E) : 0u;
     }
+    // this thread's first row and its element of a row
+    static __device__ __forceinline__ int first_row(int tid) { return ALL ? tid / ROW : min(tid / ROW, CH - 1); }
+    static __device__ __forceinline__ int first_at(int tid) { return (tid % ROW) * PER; }
     // steps first .. first + 63 of n > first
-    __device__ __forceinline__ void load(int first) {
+    __device__ __forceinline__ void load(int first, int tid) {
+        const int row0 = first_row(tid), at0 = first_at(tid);
         const int left = n - first, low = reverse ? left - CH : first;          // memory row of the chunk's first row (can be below 0)
         const int row_min = reverse ? max(CH - left, 0) : 0, row_max = reverse ? CH - 1 : min(left, CH) - 1;
         const char* at = reinterpret_cast<const char*>(base + (int64_t)low * stride);
         if (FULL && left >= CH) {
+            const unsigned off0 = (unsigned)row0 * (unsigned)((int)stride * (int)sizeof(E)) + (unsigned)at0 * (unsigned)sizeof(E);
 #pragma unroll
             for (int q = 0; q < N; ++q) v[q] = row16<E>::load(reinterpret_cast<const E*>(at + (int64_t)(q * STEP) * stride * (int)sizeof(E) + off0));
         } else {
@@ -194,6 +220,7 @@ struct mix_stage_t {
         }
     }
     __device__ __forceinline__ void store(E* lds, int left, int tid) {
+        const int row0 = first_row(tid), at0 = first_at(tid);
         if (!FULL || left < CH) {
 #pragma unroll
             for (int q = 0; q < N; ++q) {
@@ -218,29 +245,32 @@ struct mix_stage_t {
     }
 };
 
-template <typename E, int DA, int NW>
+template <typename E, int TS, int DA, int NW>
 struct mix_geom {
-    static constexpr int DC = 16 * NW, NT = 64 * NW, SA = DA + mix_ops<E>::PAD, SC = DC + mix_ops<E>::PAD, SP = CH + mix_ops<E>::PAD;
-    static constexpr int A = 0, B = A + CH * SA, C = B + CH * SA, P = C + CH * SC, END = P + mix_ops<E>::P_PARTS * CH * SP;
+    typedef mix_ops<E, TS> M;
+    static constexpr int DC = TS * NW, NT = 64 * NW, SA = DA + M::PAD, SC = DC + M::PAD, SP = CH + M::PAD;
+    static constexpr int A = 0, B = A + CH * SA, C = B + CH * SA, P = C + CH * SC, END = P + M::P_PARTS * CH * SP;
     static constexpr int BYTES = END * (int)sizeof(E);
     static constexpr int FIT = NW * (160 * 1024 / (BYTES + 2048)), MIN_WAVES = FIT >= 8 ? 2 : 1;      // waves of a compute unit, and so of a SIMD, that LDS has room for
 };
 
-template <typename E, int DA, int NW, bool FULL>
-__global__ void __launch_bounds__(64 * NW, (mix_geom<E, DA, NW>::MIN_WAVES)) linattn_mix_kernel(mix_t p) {
-    typedef mix_ops<E> M;
-    typedef mix_geom<E, DA, NW> G;
+template <typename E, int TS, int DA, int NW, bool FULL>
+__global__ void __launch_bounds__(64 * NW, (mix_geom<E, TS, DA, NW>::MIN_WAVES)) linattn_mix_kernel(mix_t p) {
+    typedef mix_ops<E, TS> M;
+    typedef mix_geom<E, TS, DA, NW> G;
     typedef typename M::frag frag;
-    constexpr int NT = G::NT, TILES = DA / 16, NPA = DA / M::KB, NPC = CH / M::KB, TPP = M::KB / 16;     // fragments over DA, over a chunk; tiles of one
+    typedef typename M::acc acc;
+    constexpr int NT = G::NT, TILES = DA / TS, IT = CH / TS, NPA = DA / M::KB, NPC = CH / M::KB;       // tiles of S and of O; fragments over DA, over a chunk
+    constexpr int AR = TS * TS / 64, QUADS = AR / 4;               // a lane's values of a tile, in runs of four neighbouring rows: 8 quad + 4 g (32) or 4 g
     constexpr int PLANE = CH * G::SP;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds_raw[];
     E* la = reinterpret_cast<E*>(lds_raw) + G::A;
     E* lb = reinterpret_cast<E*>(lds_raw) + G::B;
     E* lc = reinterpret_cast<E*>(lds_raw) + G::C;
     E* lp = reinterpret_cast<E*>(lds_raw) + G::P;
-    // powers of lam: 0..64 and that of the last chunk's steps; those of the scores by i - j + 16, 0 for i < j; weights of a S and of c by step, of
+    // powers of lam: 0..64 and that of the last chunk's steps; those of the scores by i - j + 32, 0 for i < j; weights of a S and of c by step, of
     // whole chunks without a cut [0] and of the chunk at hand otherwise [1]
-    __shared__ float pw[CH + 2], pw_low[CH + 2], score_w[CH + 16], wq[2][CH], wb[2][CH];
+    __shared__ float pw[CH + 2], pw_low[CH + 2], score_w[CH + 32], wq[2][CH], wb[2][CH];
     __shared__ int seg_of[CH];
     // workgroups of one row and head follow each other on one XCD (ids go round the 8 of them): its jobs share their reads in that L2
     const int lin = blockIdx.x, turn = lin >> 3, both = turn % (p.n_jobs * p.n_slices);
@@ -248,8 +278,9 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, DA, NW>::MIN_WAVES)) lin
     if (unit >= p.B * p.H * p.n_seg) return;
     const mix_job_t& J = p.job[job_i];
     const int bh = unit / p.n_seg, seg = unit % p.n_seg, b = bh / p.H, h = bh % p.H;
-    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), ln = lane & 15, g = lane >> 4;
-    const int n = p.lengths ? min(max(p.lengths[b], 0), p.T) : p.T;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), ln0 = lane % TS, g0 = lane / TS;
+    typedef const __attribute__((address_space(4))) int* scalar_int_t;
+    const int n = p.lengths ? min(max(((scalar_int_t)(uintptr_t)p.lengths)[b], 0), p.T) : p.T;
     const int c_first = seg * p.seg_chunks, c_end = min(c_first + p.seg_chunks, (n + CH - 1) / CH);
     const int c0 = (both % p.n_slices) * G::DC;                     // the slice of c's columns
     const int da = FULL ? DA : J.da, dc = FULL ? G::DC : min(J.dc - c0, G::DC), reverse = J.reverse, off = J.off;
@@ -260,26 +291,26 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, DA, NW>::MIN_WAVES)) lin
     E* po = (E*)J.out + b * J.so[1] + h * J.so[2] + c0;
     const int64_t so = J.so[0];
 
-    mix_stage_t<E, DA, NT, FULL> ra, rb;
-    mix_stage_t<E, G::DC, NT, FULL> rc;
-    ra.begin((const E*)J.a + b * J.sa[1] + h * J.sa[2], J.sa[0], da, n, reverse, tid);
-    rb.begin((const E*)J.b + b * J.sb[1] + h * J.sb[2], J.sb[0], da, n, reverse, tid);
-    rc.begin((const E*)J.c + b * J.sc[1] + h * J.sc[2] + c0, J.sc[0], dc, n, reverse, tid);
+    mix_stage_t<E, DA, NT, FULL, M::PAD> ra, rb;
+    mix_stage_t<E, G::DC, NT, FULL, M::PAD> rc;
+    ra.begin((const E*)J.a + b * J.sa[1] + h * J.sa[2], J.sa[0], da, n, reverse);
+    rb.begin((const E*)J.b + b * J.sb[1] + h * J.sb[2], J.sb[0], da, n, reverse);
+    rc.begin((const E*)J.c + b * J.sc[1] + h * J.sc[2] + c0, J.sc[0], dc, n, reverse);
     float rflag = 0.f;
-    auto request = [&](int c) {
+    auto request = [&](int c, int tid) {
         const int first = c * CH;
-        if (!states_only) ra.load(first);
-        rb.load(first);
-        rc.load(first);
+        if (!states_only) ra.load(first, tid);
+        rb.load(first, tid);
+        rc.load(first, tid);
         if (reset) {
             // what came before step i is cut off: by the reset of step i; in reversed time by that of the step behind it
             const int i = first + lane, t = reverse ? n - i : i;
             rflag = reset[(int64_t)min(max(t, 0), n - 1) * p.B + b];           // of another step where there is none: see below
         }
     };
-    if (c_first < c_end) request(c_first);
-
-    float gl = p.log_decay[h];
+    typedef const __attribute__((address_space(4))) float* scalar_t;
+    float gl = ((scalar_t)(uintptr_t)p.log_decay)[h];               // before the rows are requested: vector loads come back in order
+    if (c_first < c_end) request(c_first, tid);
     gl = gl > 0.f ? 0.f : gl < -1e30f ? -1e30f : gl;
     const int n_last = n - (n - 1) / CH * CH;                       // steps of the row's last chunk (n > 0)
     for (int k = tid; k < CH + 2; k += NT) {
@@ -287,20 +318,22 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, DA, NW>::MIN_WAVES)) lin
         pw[k] = (float)f;
         pw_low[k] = (float)(f - (double)(float)f);
     }
-    f32x4_t S[TILES];
+    acc S[TILES];
     {
         const float* s = J.s_in;
-        const int e = 16 * w + ln;
+        const int e = TS * w + ln0;
 #pragma unroll
-        for (int t = 0; t < TILES; ++t) S[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < TILES; ++t)
+#pragma unroll
+            for (int r = 0; r < AR; ++r) S[t][r] = 0.f;
         if (s) {
             s += ((int64_t)bh * p.n_seg + seg) * J.s_row + (c0 + e) * J.se;
             const int sd = J.sd;
 #pragma unroll
             for (int t = 0; t < TILES; ++t)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int d = 16 * t + 4 * g + r;
+                for (int r = 0; r < AR; ++r) {
+                    const int d = TS * t + 8 * (r >> 2) + 4 * g0 + (r & 3);
                     if (FULL || (d < da && e < dc)) S[t][r] = s[d * sd];
                 }
         }
@@ -308,7 +341,7 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, DA, NW>::MIN_WAVES)) lin
     const bool fine = states_only || (J.s_out && p.n_seg == 1);      // the state is a result
     if (!states_only) {
         // P's tiles above the diagonal that share a fragment with one on it are read and stay 0
-        if (TPP == 2)
+        if (M::KB > TS)
             for (int at = tid; at < 32 * M::P_PARTS; at += NT) {
                 const int i = ((at >> 4) & 1) * 32 + (at & 15);                           // rows 0..15 and 32..47
                 u32x4_t* z = reinterpret_cast<u32x4_t*>(lp + (at >> 5) * PLANE + i * G::SP + (i & 32) + 16);
@@ -327,7 +360,7 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, DA, NW>::MIN_WAVES)) lin
         }
     }
     lds_barrier();
-    for (int k = tid; k < CH + 16; k += NT) score_w[k] = k < 16 ? 0.f : scale_p * pw[max(k - 16, 0)];
+    for (int k = tid; k < CH + 32; k += NT) score_w[k] = k < 32 ? 0.f : scale_p * pw[k - 32];
     if (tid < CH) {
         wq[0][tid] = scale_s * pw[tid + off];
         wb[0][tid] = scale_b * pw[CH - tid - off];
@@ -336,15 +369,17 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, DA, NW>::MIN_WAVES)) lin
     bool cut_any = false;
     for (int c = c_first; c < c_end; ++c) {
         const int left = n - c * CH;
+        int ln = ln0, g = g0, tx = tid;
+        asm volatile("" : "+v"(ln), "+v"(g), "+v"(tx));             // addresses are made anew: kept over the loop they would not fit the registers
         unsigned long long cuts = 0;
         if (reset) {
             const int i = c * CH + lane;
             cuts = __ballot(rflag != 0.f && i < n && (!reverse || i > 0));
         }
         cut_any = cut_any || cuts != 0;
-        if (!states_only) ra.store(la, left, tid);
-        rb.store(lb, left, tid);
-        rc.store(lc, left, tid);
+        if (!states_only) ra.store(la, left, tx);
+        rb.store(lb, left, tx);
+        rc.store(lc, left, tx);
         const int own_w = cuts != 0 || left < CH ? 1 : 0;
         if (own_w && tid < CH) {
             const int nv = min(left, CH), k = __popcll(cuts & (~0ull >> (63 - tid)));      // cuts up to and including this step
@@ -354,25 +389,26 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, DA, NW>::MIN_WAVES)) lin
             wb[1][tid] = tid < nv && k == __popcll(cuts) ? scale_b * x : 0.f;
         }
         lds_barrier();
-        if (c + 1 < c_end) request(c + 1);
-        f32x4_t O[4];
+        if (c + 1 < c_end) request(c + 1, tx);
+        acc O[IT];
         if (!states_only) {
             // P^T tiles on and below the diagonal, dealt out to the waves, up to three at a time
-            constexpr int MINE = (10 + NW - 1) / NW, AT_ONCE = MINE < 3 ? MINE : 3;
+            constexpr int ALL_P = IT * (IT + 1) / 2, MINE = (ALL_P + NW - 1) / NW, AT_ONCE = MINE < 3 ? MINE : 3;
 #pragma unroll
             for (int t0 = 0; t0 < MINE; t0 += AT_ONCE) {
-                f32x4_t s[AT_ONCE];
+                acc s[AT_ONCE];
                 int it[AT_ONCE], jt[AT_ONCE];
                 const E *ax[AT_ONCE], *bx[AT_ONCE];
-                float sw[AT_ONCE][4];
+                float sw[AT_ONCE][AR];
 #pragma unroll
                 for (int k = 0; k < AT_ONCE; ++k) {
-                    const int t = min(w + (t0 + k) * NW, 9);                          // a wave without one repeats the last: the same values again
+                    const int t = min(w + (t0 + k) * NW, ALL_P - 1);                  // a wave without one repeats the last: the same values again
                     it[k] = t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3;
                     jt[k] = t - it[k] * (it[k] + 1) / 2;
-                    s[k] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-                    ax[k] = la + (16 * it[k] + ln) * G::SA;
-                    bx[k] = lb + (16 * jt[k] + ln) * G::SA;
+#pragma unroll
+                    for (int r = 0; r < AR; ++r) s[k][r] = 0.f;
+                    ax[k] = la + (TS * it[k] + ln) * G::SA;
+                    bx[k] = lb + (TS * jt[k] + ln) * G::SA;
                 }
                 frag fa[2][AT_ONCE], fb[2][AT_ONCE];
 #pragma unroll
@@ -384,7 +420,7 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, DA, NW>::MIN_WAVES)) lin
 #pragma unroll
                         for (int k = 0; k < AT_ONCE; ++k)
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) sw[k][r] = score_w[16 + 16 * (it[k] - jt[k]) + ln - 4 * g - r];
+                            for (int r = 0; r < AR; ++r) sw[k][r] = (score_w + (5 + ln - 4 * g + TS * (it[k] - jt[k])))[27 - 8 * (r >> 2) - (r & 3)];
                     }
                     if (q > 0) {
 #pragma unroll
@@ -393,33 +429,40 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, DA, NW>::MIN_WAVES)) lin
                             for (int k = 0; k < AT_ONCE; ++k)
                                 if (t0 + k < MINE) s[k] = M::mfma(fb[(q - 1) & 1][k], fa[(q - 1) & 1][k], s[k], x);
                     }
+                    if (TS == 32) __builtin_amdgcn_sched_barrier(0);    // fragments of two steps at a time: more do not fit the registers
                 }
 #pragma unroll
                 for (int k = 0; k < AT_ONCE; ++k)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) s[k][r] *= sw[k][r];
+                    for (int r = 0; r < AR; ++r) s[k][r] *= sw[k][r];
                 if (cuts) {
 #pragma unroll
                     for (int k = 0; k < AT_ONCE; ++k) {
-                        const int m = seg_of[16 * it[k] + ln];
+                        const int m = seg_of[TS * it[k] + ln];
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) s[k][r] = seg_of[16 * jt[k] + 4 * g + r] == m ? s[k][r] : 0.f;
+                        for (int r = 0; r < AR; ++r) s[k][r] = seg_of[TS * jt[k] + 8 * (r >> 2) + 4 * g + (r & 3)] == m ? s[k][r] : 0.f;
                     }
                 }
 #pragma unroll
                 for (int k = 0; k < AT_ONCE; ++k)
-                    if (t0 + k < MINE) M::store_p(lp + (16 * it[k] + ln) * G::SP + 16 * jt[k] + 4 * g, PLANE, s[k]);
+#pragma unroll
+                    for (int x = 0; x < QUADS; ++x)
+                        if (t0 + k < MINE)
+                            M::store_p(lp + (TS * it[k] + ln) * G::SP + TS * jt[k] + 8 * x + 4 * g, PLANE,
+                                       f32x4_t{s[k][4 * x], s[k][4 * x + 1], s[k][4 * x + 2], s[k][4 * x + 3]});
             }
 #pragma unroll
-            for (int it = 0; it < 4; ++it) O[it] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-            frag fa[2][4];
-            float fq[4];
+            for (int it = 0; it < IT; ++it)
+#pragma unroll
+                for (int r = 0; r < AR; ++r) O[it][r] = 0.f;
+            frag fa[2][IT];
+            float fq[IT];
 #pragma unroll
             for (int q = 0; q <= NPA; ++q) {
 #pragma unroll
-                for (int it = 0; it < 4; ++it) {
-                    if (q < NPA) fa[q & 1][it] = M::row(la + (16 * it + ln) * G::SA, q, g);
-                    else fq[it] = wq[own_w][16 * it + ln];
+                for (int it = 0; it < IT; ++it) {
+                    if (q < NPA) fa[q & 1][it] = M::row(la + (TS * it + ln) * G::SA, q, g);
+                    else fq[it] = wq[own_w][TS * it + ln];
                 }
                 if (q > 0) {
                     frag fs[M::S_PARTS];
@@ -429,13 +472,14 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, DA, NW>::MIN_WAVES)) lin
 #pragma unroll
                         for (int x = 0; x < M::STEPS; ++x)
 #pragma unroll
-                            for (int it = 0; it < 4; ++it) O[it] = M::mfma(fs[part], fa[(q - 1) & 1][it], O[it], x);
+                            for (int it = 0; it < IT; ++it) O[it] = M::mfma(fs[part], fa[(q - 1) & 1][it], O[it], x);
                 }
+                if (TS == 32) __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
-            for (int it = 0; it < 4; ++it)
+            for (int it = 0; it < IT; ++it)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) O[it][r] *= fq[it];
+                for (int r = 0; r < AR; ++r) O[it][r] *= fq[it];
             lds_barrier();
         }
         {
@@ -446,38 +490,38 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, DA, NW>::MIN_WAVES)) lin
 #pragma unroll
                 for (int t = 0; t < TILES; ++t)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) S[t][r] = __builtin_fmaf(S[t][r], ch, S[t][r] * cl);
+                    for (int r = 0; r < AR; ++r) S[t][r] = __builtin_fmaf(S[t][r], ch, S[t][r] * cl);
             } else {
 #pragma unroll
                 for (int t = 0; t < TILES; ++t)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) S[t][r] *= ch;
+                    for (int r = 0; r < AR; ++r) S[t][r] *= ch;
             }
         }
 #pragma unroll
         for (int q = 0; q < NPC; ++q) {
-            const frag cf = M::column(lc, G::SC, q, g, 16 * w + ln);
-            frag cw[M::W_PARTS], fp[M::P_PARTS][4], fb[TILES];
-            float wv[M::KB / 4];
+            const frag cf = M::column(lc, G::SC, q, g, TS * w + ln);
+            frag cw[M::W_PARTS], fp[M::P_PARTS][IT], fb[TILES];
+            float wv[M::SLOTS];
 #pragma unroll
-            for (int r = 0; r < M::KB / 4; ++r) wv[r] = wb[own_w][M::KB * q + (M::KB / 4) * g + r];
+            for (int r = 0; r < M::SLOTS; ++r) wv[r] = wb[own_w][M::KB * q + M::SLOTS * g + r];
             if (!states_only) {
 #pragma unroll
                 for (int part = 0; part < M::P_PARTS; ++part)
 #pragma unroll
-                    for (int it = 0; it < 4; ++it)
-                        if (q * TPP <= it) fp[part][it] = M::row_natural(lp + part * PLANE + (16 * it + ln) * G::SP, q, g);
+                    for (int it = 0; it < IT; ++it)
+                        if (q * M::KB < TS * (it + 1)) fp[part][it] = M::row_natural(lp + part * PLANE + (TS * it + ln) * G::SP, q, g);
             }
 #pragma unroll
-            for (int t = 0; t < TILES; ++t) fb[t] = M::column(lb, G::SA, q, g, 16 * t + ln);
+            for (int t = 0; t < TILES; ++t) fb[t] = M::column(lb, G::SA, q, g, TS * t + ln);
             if (!states_only) {
 #pragma unroll
                 for (int part = M::P_PARTS - 1; part >= 0; --part)
 #pragma unroll
                     for (int x = 0; x < M::STEPS; ++x)
 #pragma unroll
-                        for (int it = 0; it < 4; ++it)
-                            if (q * TPP <= it) O[it] = M::mfma(cf, fp[part][it], O[it], x);
+                        for (int it = 0; it < IT; ++it)
+                            if (q * M::KB < TS * (it + 1)) O[it] = M::mfma(cf, fp[part][it], O[it], x);
             }
             M::weigh(cf, wv, cw, fine);
 #pragma unroll
@@ -488,33 +532,37 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, DA, NW>::MIN_WAVES)) lin
 #pragma unroll
                     for (int t = 0; t < TILES; ++t) S[t] = M::mfma(fb[t], cw[part], S[t], x);
             }
+            if (TS == 32) __builtin_amdgcn_sched_barrier(0);
         }
         if (!states_only) {
             // rows of O in the order of memory, as the stage's
-            const int low = reverse ? left - CH : c * CH, e = 16 * w + 4 * g;
-            E* at = po + (int64_t)low * so + (int64_t)(reverse ? 15 - ln : ln) * so + e;
+            const int low = reverse ? left - CH : c * CH, e = TS * w + 4 * g;
+            E* at = po + (int64_t)low * so + (int64_t)(reverse ? TS - 1 - ln : ln) * so + e;
 #pragma unroll
-            for (int it = 0; it < 4; ++it) {
-                E* o = at + (int64_t)(16 * (reverse ? 3 - it : it)) * so;
-                if (16 * it + ln < left) {
-                    if (FULL || e + 4 <= dc) M::store_out(o, O[it]);
-                    else
+            for (int it = 0; it < IT; ++it) {
+                E* o = at + (int64_t)(TS * (reverse ? IT - 1 - it : it)) * so;
+                if (TS * it + ln < left) {
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) if (e + r < dc) io_store(o + r, O[it][r]);
+                    for (int x = 0; x < QUADS; ++x) {
+                        if (FULL || e + 8 * x + 4 <= dc) M::store_out(o + 8 * x, f32x4_t{O[it][4 * x], O[it][4 * x + 1], O[it][4 * x + 2], O[it][4 * x + 3]});
+                        else
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) if (e + 8 * x + r < dc) io_store(o + 8 * x + r, O[it][4 * x + r]);
+                    }
                 }
             }
         }
         lds_barrier();
     }
-    const int e = 16 * w + ln;
+    const int e = TS * w + ln0;
     if (states_only) {
         const int64_t at = ((int64_t)bh * p.n_seg + seg);
         float* s = J.s_out + at * p.kv + c0;
 #pragma unroll
-        for (int t = 0; t < DA / 16; ++t)
+        for (int t = 0; t < TILES; ++t)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int d = 16 * t + 4 * g + r;
+            for (int r = 0; r < AR; ++r) {
+                const int d = TS * t + 8 * (r >> 2) + 4 * g0 + (r & 3);
                 if (d < da && e < dc) s[d * J.dc + e] = S[t][r];
             }
         if (tid == 0 && c0 == 0) {
@@ -526,44 +574,44 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, DA, NW>::MIN_WAVES)) lin
     } else if (J.s_out && p.n_seg == 1) {
         const bool none = J.off == 0 && n > 0 && p.reset && p.reset[b] != 0.f;      // the gradient stops at a reset before the first step
 #pragma unroll
-        for (int t = 0; t < DA / 16; ++t)
+        for (int t = 0; t < TILES; ++t)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int d = 16 * t + 4 * g + r;
+            for (int r = 0; r < AR; ++r) {
+                const int d = TS * t + 8 * (r >> 2) + 4 * g0 + (r & 3);
                 if (d < da && e < dc) J.s_out[(int64_t)bh * p.kv + d * J.sd + (c0 + e) * J.se] = none ? 0.f : S[t][r];
             }
     }
 }
 
-template <typename E, int DA, int NW, bool FULL>
+template <typename E, int TS, int DA, int NW, bool FULL>
 static int launch_mix_as(mix_t m, int dc, hipStream_t s) {
-    typedef mix_geom<E, DA, NW> G;
+    typedef mix_geom<E, TS, DA, NW> G;
     static_assert(G::BYTES + 1500 <= 160 * 1024, "LDS");
     m.n_slices = (dc + G::DC - 1) / G::DC;
     const int64_t units = ((int64_t)m.B * m.H * m.n_seg + 7) / 8 * 8, grid = units * m.n_jobs * m.n_slices;
     XRL_CHECK_ARG(grid <= 0x7fffffff);
-    hipLaunchKernelGGL((linattn_mix_kernel<E, DA, NW, FULL>), dim3((unsigned)grid), dim3(64 * NW), G::BYTES, s, m);
+    hipLaunchKernelGGL((linattn_mix_kernel<E, TS, DA, NW, FULL>), dim3((unsigned)grid), dim3(64 * NW), G::BYTES, s, m);
     XRL_CHECK_LAUNCH();
     return XRL_OK;
 }
 
-template <typename E, int DA, int NW>
+template <typename E, int TS, int DA, int NW>
 static int launch_mix_size(const mix_t& m, int dc, hipStream_t s) {
     bool full = true;
     for (int i = 0; i < m.n_jobs; ++i) {
         const mix_job_t& j = m.job[i];
-        full = full && j.da == DA && j.dc == dc && dc % (16 * NW) == 0;
+        full = full && j.da == DA && j.dc == dc && dc % (TS * NW) == 0;
         const int64_t most = (1ll << 31) / (CH * (int)sizeof(E));
         full = full && j.sa[0] < most && j.sb[0] < most && j.sc[0] < most;
     }
-    return full ? launch_mix_as<E, DA, NW, true>(m, dc, s) : launch_mix_as<E, DA, NW, false>(m, dc, s);
+    return full ? launch_mix_as<E, TS, DA, NW, true>(m, dc, s) : launch_mix_as<E, TS, DA, NW, false>(m, dc, s);
 }
 
-template <typename E, int DA, int NW>
+template <typename E, int TS, int DA, int NW>
 static int init_mix_as() {
-    const int bytes = mix_geom<E, DA, NW>::BYTES;
-    XRL_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(linattn_mix_kernel<E, DA, NW, true>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    XRL_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(linattn_mix_kernel<E, DA, NW, false>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    const int bytes = mix_geom<E, TS, DA, NW>::BYTES;
+    XRL_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(linattn_mix_kernel<E, TS, DA, NW, true>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    XRL_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(linattn_mix_kernel<E, TS, DA, NW, false>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
     return XRL_OK;
 }
 
