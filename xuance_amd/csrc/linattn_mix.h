@@ -33,7 +33,7 @@ struct mix_t {
     mix_job_t job[3];
     const float* log_decay; const int32_t* lengths; const float* reset;
     int T, B, H, kv;
-    int n_jobs, n_seg, seg_chunks, n_slices;
+    int n_jobs, n_seg, n_slices;          // every row is cut into n_seg segments of equally many chunks, by its own length
     int states_only;                      // write every segment's own state to s_out [row and head][segment] and its carry
 };
 
@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, TS, DA, NW>::MIN_WAVES))
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), ln0 = lane % TS, g0 = lane / TS;
     typedef const __attribute__((address_space(4))) int* scalar_int_t;
     const int n = p.lengths ? min(max(((scalar_int_t)(uintptr_t)p.lengths)[b], 0), p.T) : p.T;
-    const int c_first = seg * p.seg_chunks, c_end = min(c_first + p.seg_chunks, (n + CH - 1) / CH);
+    const int seg_chunks = ((n + CH - 1) / CH + p.n_seg - 1) / p.n_seg, c_first = seg * seg_chunks, c_end = min(c_first + seg_chunks, (n + CH - 1) / CH);
     const int c0 = (both % p.n_slices) * G::DC;                     // the slice of c's columns
     const int da = FULL ? DA : J.da, dc = FULL ? G::DC : min(J.dc - c0, G::DC), reverse = J.reverse, off = J.off;
     if (!FULL && dc <= 0) return;                                   // a job of fewer columns than the widest
@@ -349,9 +349,8 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, TS, DA, NW>::MIN_WAVES))
                 z[0] = zero; z[1] = zero;
             }
         // rows behind the sequence: 0
-        const int lo = max(n, c_first * CH), hi = min(p.T, (c_first + p.seg_chunks) * CH);
         constexpr int PIECES = G::DC / 4;
-        for (int r = lo + tid / PIECES; r < hi; r += NT / PIECES) {
+        for (int r = n + seg * (NT / PIECES) + tid / PIECES; r < p.T; r += p.n_seg * (NT / PIECES)) {
             const int e = tid % PIECES * 4;
             E* o = po + (int64_t)r * so + e;
             if (e + 4 <= dc) M::store_out(o, f32x4_t{0.f, 0.f, 0.f, 0.f});
@@ -566,7 +565,7 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, TS, DA, NW>::MIN_WAVES))
                 if (d < da && e < dc) s[d * J.dc + e] = S[t][r];
             }
         if (tid == 0 && c0 == 0) {
-            const int steps = max(0, min(n, (c_first + p.seg_chunks) * CH) - c_first * CH);
+            const int steps = max(0, min(n, (c_first + seg_chunks) * CH) - c_first * CH);
             const double f = exp((double)gl * steps);
             J.carry[2 * at] = cut_any ? 0.f : (float)f;
             J.carry[2 * at + 1] = cut_any ? 0.f : (float)(f - (double)(float)f);
@@ -607,6 +606,14 @@ static int launch_mix_size(const mix_t& m, int dc, hipStream_t s) {
     return full ? launch_mix_as<E, TS, DA, NW, true>(m, dc, s) : launch_mix_as<E, TS, DA, NW, false>(m, dc, s);
 }
 
+// what a compute unit holds of an instance's workgroups
+template <typename E, int TS, int DA, int NW>
+static int mix_resident() {
+    typedef mix_geom<E, TS, DA, NW> G;
+    const int by_lds = 160 * 1024 / (G::BYTES + 2560), by_registers = 8 / NW > 0 ? 8 / NW : 1;
+    return by_lds < by_registers ? by_lds : by_registers;
+}
+
 template <typename E, int TS, int DA, int NW>
 static int init_mix_as() {
     const int bytes = mix_geom<E, TS, DA, NW>::BYTES;
@@ -619,5 +626,7 @@ int launch_mix_f32(const mix_t& m, int da, int dc, hipStream_t s);
 int launch_mix_bf16(const mix_t& m, int da, int dc, hipStream_t s);
 int init_mix_f32();
 int init_mix_bf16();
+int mix_resident_f32(int da, int dc);
+int mix_resident_bf16(int da, int dc);
 
 }  // namespace xrl
