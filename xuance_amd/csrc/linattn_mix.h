@@ -254,6 +254,19 @@ struct mix_geom {
     static constexpr int FIT = NW * (160 * 1024 / (BYTES + 2048)), MIN_WAVES = FIT >= 8 ? 2 : 1;      // waves of a compute unit, and so of a SIMD, that LDS has room for
 };
 
+// between scheduling fences: V vector instructions behind each of N matrix instructions, which run meanwhile
+template <int N, int V>
+__device__ __forceinline__ void mix_interleave(bool both) {
+    if (both) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, V, 0);
+        }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+}
+
 template <typename E, int TS, int DA, int NW, bool FULL>
 __global__ void __launch_bounds__(64 * NW, (mix_geom<E, TS, DA, NW>::MIN_WAVES)) linattn_mix_kernel(mix_t p) {
     typedef mix_ops<E, TS> M;
@@ -454,26 +467,25 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, TS, DA, NW>::MIN_WAVES))
             for (int it = 0; it < IT; ++it)
 #pragma unroll
                 for (int r = 0; r < AR; ++r) O[it][r] = 0.f;
-            frag fa[2][IT];
+            frag fa[2][IT], fs[2][M::S_PARTS];
             float fq[IT];
 #pragma unroll
-            for (int q = 0; q <= NPA; ++q) {
+            for (int q = -1; q < NPA; ++q) {                                          // the next fragments are made while these are multiplied
 #pragma unroll
                 for (int it = 0; it < IT; ++it) {
-                    if (q < NPA) fa[q & 1][it] = M::row(la + (TS * it + ln) * G::SA, q, g);
+                    if (q + 1 < NPA) fa[(q + 1) & 1][it] = M::row(la + (TS * it + ln) * G::SA, q + 1, g);
                     else fq[it] = wq[own_w][TS * it + ln];
                 }
-                if (q > 0) {
-                    frag fs[M::S_PARTS];
-                    M::of_state(S, q - 1, fs);
+                if (q >= 0) {
 #pragma unroll
                     for (int part = M::S_PARTS - 1; part >= 0; --part)
 #pragma unroll
                         for (int x = 0; x < M::STEPS; ++x)
 #pragma unroll
-                            for (int it = 0; it < IT; ++it) O[it] = M::mfma(fs[part], fa[(q - 1) & 1][it], O[it], x);
+                            for (int it = 0; it < IT; ++it) O[it] = M::mfma(fs[q & 1][part], fa[q & 1][it], O[it], x);
                 }
-                if (TS == 32) __builtin_amdgcn_sched_barrier(0);
+                if (q + 1 < NPA) M::of_state(S, q + 1, fs[(q + 1) & 1]);
+                if (TS == 32) mix_interleave<IT * M::S_PARTS, 6>(q >= 0 && q + 1 < NPA);
             }
 #pragma unroll
             for (int it = 0; it < IT; ++it)
@@ -481,57 +493,64 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, TS, DA, NW>::MIN_WAVES))
                 for (int r = 0; r < AR; ++r) O[it][r] *= fq[it];
             lds_barrier();
         }
-        {
-            const bool last = left <= CH;
-            const float ch = cuts ? 0.f : pw[last ? CH + 1 : CH], cl = cuts ? 0.f : pw_low[last ? CH + 1 : CH];
-            // where half of the state or more is gone a chunk later, the rounding of lam^64 does not add up over the chunks
-            if (__builtin_amdgcn_readfirstlane(ch > 0.5f)) {
+        const bool last = left <= CH;
+        const float ch = cuts ? 0.f : pw[last ? CH + 1 : CH], cl = cuts ? 0.f : pw_low[last ? CH + 1 : CH];
+        // where half of the state or more is gone a chunk later, the rounding of lam^64 does not add up over the chunks
+        const bool two = __builtin_amdgcn_readfirstlane(ch > 0.5f);
+        frag cf[NPC];
 #pragma unroll
-                for (int t = 0; t < TILES; ++t)
+        for (int q = 0; q < NPC; ++q) cf[q] = M::column(lc, G::SC, q, g, TS * w + ln);
 #pragma unroll
-                    for (int r = 0; r < AR; ++r) S[t][r] = __builtin_fmaf(S[t][r], ch, S[t][r] * cl);
-            } else {
-#pragma unroll
-                for (int t = 0; t < TILES; ++t)
-#pragma unroll
-                    for (int r = 0; r < AR; ++r) S[t][r] *= ch;
-            }
-        }
-#pragma unroll
-        for (int q = 0; q < NPC; ++q) {
-            const frag cf = M::column(lc, G::SC, q, g, TS * w + ln);
-            frag cw[M::W_PARTS], fp[M::P_PARTS][IT], fb[TILES];
-            float wv[M::SLOTS];
-#pragma unroll
-            for (int r = 0; r < M::SLOTS; ++r) wv[r] = wb[own_w][M::KB * q + M::SLOTS * g + r];
-            if (!states_only) {
+        for (int q = 0; q < (NPC > TILES ? NPC : TILES); ++q) {
+            if (q < NPC && !states_only) {
+                frag fp[M::P_PARTS][IT];
 #pragma unroll
                 for (int part = 0; part < M::P_PARTS; ++part)
 #pragma unroll
                     for (int it = 0; it < IT; ++it)
                         if (q * M::KB < TS * (it + 1)) fp[part][it] = M::row_natural(lp + part * PLANE + (TS * it + ln) * G::SP, q, g);
-            }
-#pragma unroll
-            for (int t = 0; t < TILES; ++t) fb[t] = M::column(lb, G::SA, q, g, TS * t + ln);
-            if (!states_only) {
 #pragma unroll
                 for (int part = M::P_PARTS - 1; part >= 0; --part)
 #pragma unroll
                     for (int x = 0; x < M::STEPS; ++x)
 #pragma unroll
                         for (int it = 0; it < IT; ++it)
-                            if (q * M::KB < TS * (it + 1)) O[it] = M::mfma(cf, fp[part][it], O[it], x);
+                            if (q * M::KB < TS * (it + 1)) O[it] = M::mfma(cf[q], fp[part][it], O[it], x);
             }
-            M::weigh(cf, wv, cw, fine);
+            if (q < TILES) {
+                if (two) {
 #pragma unroll
-            for (int part = M::W_PARTS - 1; part >= 0; --part) {
-                if (part == 2 && !fine) continue;
+                    for (int r = 0; r < AR; ++r) S[q][r] = __builtin_fmaf(S[q][r], ch, S[q][r] * cl);
+                } else {
 #pragma unroll
-                for (int x = 0; x < M::STEPS; ++x)
-#pragma unroll
-                    for (int t = 0; t < TILES; ++t) S[t] = M::mfma(fb[t], cw[part], S[t], x);
+                    for (int r = 0; r < AR; ++r) S[q][r] *= ch;
+                }
             }
-            if (TS == 32) __builtin_amdgcn_sched_barrier(0);
+        }
+        frag cw[2][M::W_PARTS];
+#pragma unroll
+        for (int q = -1; q < NPC; ++q) {
+            frag fb[TILES];
+            if (q >= 0)
+#pragma unroll
+                for (int t = 0; t < TILES; ++t) fb[t] = M::column(lb, G::SA, q, g, TS * t + ln);
+            float wv[M::SLOTS];
+            if (q + 1 < NPC) {
+#pragma unroll
+                for (int r = 0; r < M::SLOTS; ++r) wv[r] = wb[own_w][M::KB * (q + 1) + M::SLOTS * g + r];
+            }
+            if (q >= 0) {
+#pragma unroll
+                for (int part = M::W_PARTS - 1; part >= 0; --part) {
+                    if (part == 2 && !fine) continue;
+#pragma unroll
+                    for (int x = 0; x < M::STEPS; ++x)
+#pragma unroll
+                        for (int t = 0; t < TILES; ++t) S[t] = M::mfma(fb[t], cw[q & 1][part], S[t], x);
+                }
+            }
+            if (q + 1 < NPC) M::weigh(cf[q + 1], wv, cw[(q + 1) & 1], fine);
+            if (TS == 32) mix_interleave<TILES * 2, 7>(q >= 0 && q + 1 < NPC);
         }
         if (!states_only) {
             // rows of O in the order of memory, as the stage's
