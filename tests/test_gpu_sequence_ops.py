@@ -720,6 +720,53 @@ def test_distill_lowest_values_and_repeated_entries(ops, A):
     distill_check(ops, c)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("K", [8, 100, 256])
+@pytest.mark.parametrize("A", [30, 100, 500, 3000, 11000, 20000, 70000])
+def test_distill_entries_near_each_other(ops, A, K, dtype):
+    """Entries of one action and of neighbouring actions, which one lane or thread holds together."""
+    c = distill_case(8, 5, A, K, dtype)
+    order = torch.randperm(K, generator=gen(9))
+    c["teacher_idx"][0] = (7 + order % 4).int()                 # four actions side by side, named K / 4 times
+    c["teacher_idx"][1] = (3 + order % min(24, A - 3)).int()    # more than a lane holds
+    c["teacher_idx"][2] = A - 1 - (order % 3).int()             # the last three
+    c["teacher_idx"][3] = torch.where(order % 2 == 0, torch.tensor(A // 2), torch.tensor(-5)).int()
+    distill_check(ops, c)
+    distill_check(ops, c, layout=odd_rows)
+
+
+@pytest.mark.parametrize("A", [500, 11000, 20000, 70000])
+def test_distill_rows_with_nothing_at_other_sizes(ops, A):
+    c = distill_case(12, 6, A, 5, avail=True)
+    c["weight"][:] = 1.0
+    c["avail"][0] = 0.0
+    c["teacher_idx"][1] = A
+    c["avail"][2].scatter_(0, c["teacher_idx"][2].long(), 0.0)
+    c["weight"][3] = 0.0
+    c["logits"][3] = math.nan
+    c["logits"][4] = -math.inf
+    loss, d = distill_check(ops, c)
+    assert (loss[:5] == 0).all() and (d[:5] == 0).all() and loss[5] != 0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("A", [30, 500, 3000, 20000, 70000])
+def test_distill_nan_reaches_the_result(ops, A, dtype):
+    """A NaN among a row's logits, a row of nothing else, a NaN of the teacher: that row's loss is NaN, the others are as before."""
+    c = distill_case(13, 6, A, 5, dtype)
+    want = distill_run(ops, c, 2.0, 0.5)
+    c["logits"][1, A // 3] = math.nan
+    c["logits"][2] = math.nan
+    c["teacher_logits"][4, 2] = math.nan
+    loss, d = distill_run(ops, c, 2.0, 0.5)
+    for row in range(6):
+        if row in (1, 2, 4):
+            assert torch.isnan(loss[row])
+            assert torch.isnan(d[row].float()).all() if row != 4 else torch.isnan(d[row, c["teacher_idx"][4].long().cuda()].float()).all()
+        else:
+            assert torch.equal(loss[row], want[0][row]) and torch.equal(d[row], want[1][row])
+
+
 def test_distill_layout_in_place_and_loss_only(ops):
     for A, K in ((18, 6), (700, 30), (5000, 12)):
         c = distill_case(5, 9, A, K, avail=True)
