@@ -12,6 +12,17 @@
 namespace xrl {
 
 constexpr int NV = 8;                  // values of a row per lane
+
+// The build keeps products and sums apart (-ffp-contract=off); here they are fused by hand, a third of the vector instructions, which come close to
+// the memory's time for 16-bit rows.
+__device__ __forceinline__ float fma_f(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
+
+// act_apply_c with the sigmoid from v_exp_f32 and v_rcp_f32 (a unit in the last place each) instead of expf and a division
+template <int ACT>
+__device__ __forceinline__ float gate_act_c(float z) {
+    if (ACT == XRL_ACT_SIGMOID) return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * z));
+    return act_apply_c<ACT>(z);
+}
 constexpr int NORM_SUMS = 5;           // d_scale, d_w_post, d_b_post, d_w_pre, d_b_pre
 
 template <int L>
@@ -110,8 +121,8 @@ __device__ __forceinline__ float normalize(float (&v)[NV], int at, int D, float 
     }
     float q = 0.f;
 #pragma unroll
-    for (int m = 0; m < NV; ++m) q += v[m] * v[m];
-    const float r = 1.f / sqrtf(sum(q) * inv_d + eps);
+    for (int m = 0; m < NV; ++m) q = fma_f(v[m], v[m], q);
+    const float r = 1.f / sqrtf(fma_f(sum(q), inv_d, eps));
 #pragma unroll
     for (int m = 0; m < NV; ++m) v[m] *= r;
     return r;
@@ -130,32 +141,38 @@ __global__ void __launch_bounds__(norm_geom<L>::THREADS) block_norm_fwd_kernel(x
     norm_param(p.b_post, at, D, 0.f, b0);
     norm_param(p.w_pre, at, D, 1.f, w1);
     norm_param(p.b_pre, at, D, 0.f, b1);
+    row8<E> rx, ru, rg;
+    auto request = [&](int64_t row) {
+        const int width = row < p.N ? D : 0;
+        ru.load((const E*)p.u + row * p.ld_u, at, width);
+        rx.load((const E*)p.x + row * p.ld_x, at, width);
+        if (p.gate) rg.load((const E*)p.gate + row * p.ld_gate, at, width);
+    };
+    constexpr bool AHEAD = L < 1024;                                 // 1024 threads leave no registers for it
+    if (AHEAD) request((int64_t)blockIdx.x * G::ROWS + threadIdx.x / L);
     const int64_t step = (int64_t)gridDim.x * G::ROWS;
     for (int64_t base = (int64_t)blockIdx.x * G::ROWS; base < p.N; base += step) {       // whole workgroups go round: barriers inside
         const int64_t row = base + threadIdx.x / L;
         const bool live = row < p.N;
-        const int width = live ? D : 0;
-        row8<E> rx, ru, rg;
-        ru.load((const E*)p.u + row * p.ld_u, at, width);
-        rx.load((const E*)p.x + row * p.ld_x, at, width);
-        if (p.gate) rg.load((const E*)p.gate + row * p.ld_gate, at, width);
         float x[NV], u[NV], g[NV] = {};
+        if (!AHEAD) request(row);
         ru.get(u); rx.get(x);
         if (p.gate) rg.get(g);
+        if (AHEAD && base + step < p.N) request(row + step);         // the next row is on its way while this one is worked on
         normalize<L, LN>(u, at, D, inv_d, p.eps, sum);
         if (p.gate) {
-            XRL_ACT_DISPATCH(p.gate_act, _Pragma("unroll") for (int m = 0; m < NV; ++m) g[m] = act_apply_c<ACT>(g[m]);)
+            XRL_ACT_DISPATCH(p.gate_act, _Pragma("unroll") for (int m = 0; m < NV; ++m) g[m] = gate_act_c<ACT>(g[m]);)
         }
 #pragma unroll
         for (int m = 0; m < NV; ++m) {
-            const float b = sc[m] * (u[m] * w0[m] + b0[m]);
-            x[m] += p.gate ? g[m] * b : b;
+            const float b = fma_f(u[m], w0[m], b0[m]);
+            x[m] = fma_f(p.gate ? g[m] * sc[m] : sc[m], b, x[m]);
         }
         if (live) row8<E>::store((E*)p.y + row * p.ld_y, at, D, x);
         if (p.n) {
             normalize<L, LN>(x, at, D, inv_d, p.eps, sum);
 #pragma unroll
-            for (int m = 0; m < NV; ++m) x[m] = x[m] * w1[m] + b1[m];
+            for (int m = 0; m < NV; ++m) x[m] = fma_f(x[m], w1[m], b1[m]);
             if (live) row8<E>::store((E*)p.n + row * p.ld_n, at, D, x);
         }
     }
@@ -167,11 +184,11 @@ __device__ __forceinline__ void normalize_back(float (&d)[NV], const float (&xha
                                                row_sum_t<L>& sum) {
     float a = 0.f, b = 0.f;
 #pragma unroll
-    for (int m = 0; m < NV; ++m) { a += d[m] * xhat[m]; if (LN) b += d[m]; }
+    for (int m = 0; m < NV; ++m) { a = fma_f(d[m], xhat[m], a); if (LN) b += d[m]; }
     if (LN) { const float2 t = sum(a, b); a = t.x * inv_d; b = t.y * inv_d; }
     else a = sum(a) * inv_d;
 #pragma unroll
-    for (int m = 0; m < NV; ++m) d[m] = at + m < D ? r * (d[m] - xhat[m] * a - b) : 0.f;
+    for (int m = 0; m < NV; ++m) d[m] = at + m < D ? r * fma_f(-xhat[m], a, LN ? d[m] - b : d[m]) : 0.f;
 }
 
 template <typename E, int L, bool LN>
@@ -212,17 +229,17 @@ __global__ void __launch_bounds__(norm_geom<L>::THREADS) block_norm_bwd_kernel(x
         if (AHEAD && base + step < p.N) request(row + step);
         const float ru = normalize<L, LN>(u, at, D, inv_d, p.eps, sum);
         if (p.gate) {
-            XRL_ACT_DISPATCH(p.gate_act, _Pragma("unroll") for (int m = 0; m < NV; ++m) g[m] = act_apply_c<ACT>(g[m]);)
+            XRL_ACT_DISPATCH(p.gate_act, _Pragma("unroll") for (int m = 0; m < NV; ++m) g[m] = gate_act_c<ACT>(g[m]);)
         }
+        float pm[NV];                                                // the normed block before gate and scale
+#pragma unroll
+        for (int m = 0; m < NV; ++m) pm[m] = fma_f(u[m], w0[m], b0[m]);
         if (p.d_n) {
 #pragma unroll
-            for (int m = 0; m < NV; ++m) {
-                const float b = sc[m] * (u[m] * w0[m] + b0[m]);
-                x[m] += p.gate ? g[m] * b : b;
-            }
+            for (int m = 0; m < NV; ++m) x[m] = fma_f(p.gate ? g[m] * sc[m] : sc[m], pm[m], x[m]);
             const float ry = normalize<L, LN>(x, at, D, inv_d, p.eps, sum);
 #pragma unroll
-            for (int m = 0; m < NV; ++m) { acc[3][m] += dn[m] * x[m]; acc[4][m] += dn[m]; t[m] = dn[m] * w1[m]; }
+            for (int m = 0; m < NV; ++m) { acc[3][m] = fma_f(dn[m], x[m], acc[3][m]); acc[4][m] += dn[m]; t[m] = dn[m] * w1[m]; }
             normalize_back<L, LN>(t, x, ry, at, D, inv_d, sum);
 #pragma unroll
             for (int m = 0; m < NV; ++m) dy[m] += t[m];
@@ -231,10 +248,12 @@ __global__ void __launch_bounds__(norm_geom<L>::THREADS) block_norm_bwd_kernel(x
         // y = x + scale a p: with a the activated gate
 #pragma unroll
         for (int m = 0; m < NV; ++m) {
-            const float pm = u[m] * w0[m] + b0[m], da = dy[m] * (p.gate ? g[m] : 1.f), dp = da * sc[m];
-            acc[0][m] += da * pm; acc[1][m] += dp * u[m]; acc[2][m] += dp;
+            const float da = p.gate ? dy[m] * g[m] : dy[m], dp = da * sc[m];
+            acc[0][m] = fma_f(da, pm[m], acc[0][m]);
+            acc[1][m] = fma_f(dp, u[m], acc[1][m]);
+            acc[2][m] += dp;
             t[m] = dp * w0[m];
-            dy[m] *= sc[m] * pm;                                     // gradient of the activated gate
+            dy[m] *= sc[m] * pm[m];                                  // gradient of the activated gate
         }
         if (p.d_gate) {
             XRL_ACT_DISPATCH(p.gate_act, _Pragma("unroll") for (int m = 0; m < NV; ++m) g[m] = dy[m] * act_grad_c<ACT>(g[m]);)
@@ -345,7 +364,7 @@ static void launch_norm(const xrl_block_norm_t& p, bool backward, hipStream_t s)
         using G = norm_geom<LL>;                                                                                                 \
         if (backward) hipLaunchKernelGGL((block_norm_bwd_kernel<E, LL, LN>), dim3(norm_lines(p)), dim3(G::THREADS), 0, s, p); \
         else {                                                                                                                   \
-            const int64_t need = (p.N + G::ROWS - 1) / G::ROWS, most = 2048 * 256 / G::THREADS;                                  \
+            const int64_t need = (p.N + G::ROWS - 1) / G::ROWS, most = 1024 * 256 / G::THREADS;                                  \
             hipLaunchKernelGGL((block_norm_fwd_kernel<E, LL, LN>), dim3((int)(need < most ? need : most)), dim3(G::THREADS), 0, s, p); \
         }                                                                                                                        \
     } break;
