@@ -113,11 +113,10 @@ def host_ops(monkeypatch):
             made.append(name)
         elif rc != 0:
             raise ops.XrlError(_lib.load().xrl_last_error().decode())
-    monkeypatch.setattr(ops, "_on_device", lambda t, device: True)
+    monkeypatch.setattr(ops, "_raw_stream", lambda device: None)
     monkeypatch.setattr(ops, "call", call)
     monkeypatch.setattr(ops, "init_device", lambda: None)
-    monkeypatch.setattr(ops, "stream_ptr", lambda: None)
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: -1)               # what a host tensor calls its device
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
     ops.made = made
     yield ops

@@ -1219,7 +1219,6 @@ _BLOCK_NORM = struct.Struct("@21P12q4ifi")
 _DISTILL = struct.Struct("@7P3q3iffi")
 _IO_DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 NORM_KIND = {"rms": 0, "layer": 1}
-_ROWS0 = (0, 0, 0)
 
 
 def _need(cond, what):
@@ -1227,35 +1226,23 @@ def _need(cond, what):
         raise XrlError(what)
 
 
-def _on_device(t, device):
-    return t.get_device() == device
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _wrong(name, t, shape, dtype, device):
-    if not _on_device(t, device):
-        raise XrlError(f"{name}: needs a tensor on the current device cuda:{device}, got {t.device}")
-    raise XrlError(f"{name}: needs {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
-
-
-def _dense(name, t, shape, dtype, device):
-    """-> address of a contiguous tensor (0: None) on the current device."""
-    if t is None:
-        return 0
-    if not _on_device(t, device) or t.dtype is not dtype or t.shape != shape:
-        _wrong(name, t, shape, dtype, device)
-    if not t.is_contiguous():
-        raise XrlError(f"{name}: has to be contiguous, strides are {t.stride()}")
-    return t.data_ptr()
-
-
-def _rows(name, t, shape, dtype, device):
-    """-> address and strides of a tensor on the current device whose last dimension is contiguous."""
-    if not _on_device(t, device) or t.dtype is not dtype or t.shape != shape:
-        _wrong(name, t, shape, dtype, device)
-    st = t.stride()
-    if st[-1] != 1 and shape[-1] > 1:
-        raise XrlError(f"{name}: its last dimension has to be contiguous, strides are {st}")
-    return t.data_ptr(), st[:-1]
+def _explain(device, *tensors):
+    """(name, tensor, shape, type, dense) of a call whose quick checks failed: raises for the first that is wrong; passes where none is (a last
+    dimension of one element has any stride)."""
+    for name, t, shape, dtype, dense in tensors:
+        if t is None:
+            continue
+        if t.get_device() != device:
+            raise XrlError(f"{name}: needs a tensor on the current device cuda:{device}, got {t.device}")
+        if t.dtype is not dtype or t.shape != shape:
+            raise XrlError(f"{name}: needs {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+        if dense and not t.is_contiguous():
+            raise XrlError(f"{name}: has to be contiguous, strides are {t.stride()}")
+        if not dense and t.stride(-1) != 1 and t.shape[-1] > 1:
+            raise XrlError(f"{name}: its last dimension has to be contiguous, strides are {t.stride()}")
 
 
 def _io_dtype(t):
@@ -1269,8 +1256,8 @@ def _workspace(given, floats, device):
     _lib.check(min(floats, 0), "workspace")
     if given is None:
         _need(not torch.cuda.is_current_stream_capturing(), f"a captured call needs workspace=, a float32 tensor of {floats} elements")
-        return torch.empty(floats, device=f"cuda:{device}")
-    _need(_on_device(given, device) and given.dtype is torch.float32 and given.is_contiguous() and given.numel() >= floats and
+        return torch.empty(floats, device=device)
+    _need(given.get_device() == device and given.dtype is torch.float32 and given.is_contiguous() and given.numel() >= floats and
           given.data_ptr() % 16 == 0, f"workspace: needs {floats} contiguous, 16-byte aligned float32 elements on cuda:{device}")
     return given
 
@@ -1284,7 +1271,8 @@ def linattn_workspace_floats(T, B, H, dk, dv, backward=False, dtype=torch.float3
 
 
 def _linattn_sizes(q, v):
-    init_device()
+    if not _inited:
+        init_device()
     if q.dim() != 4 or v.dim() != 4:
         raise XrlError(f"q, k, v: [T, B, H, d] each, got {tuple(q.shape)}, {tuple(v.shape)}")
     return (*q.shape, v.shape[3], _io_dtype(q), torch.cuda.current_device())
@@ -1299,20 +1287,24 @@ def linattn_forward(q, k, v, out, log_decay, scale=1.0, lengths=None, reset=None
     float32 (state_out may be state): S before the first and after the last step.  Inputs have to be finite."""
     T, B, H, dk, dv, dt, dev = _linattn_sizes(q, v)
     f32, typ, ks, vs, ss = torch.float32, q.dtype, (T, B, H, dk), (T, B, H, dv), (B, H, dk, dv)
-    pq, sq = _rows("q", q, ks, typ, dev)
-    pk, sk = _rows("k", k, ks, typ, dev)
-    pv, sv = _rows("v", v, vs, typ, dev)
-    po, so = _rows("out", out, vs, typ, dev)
-    ptrs = (pq, pk, pv, po, _dense("log_decay", log_decay, (H,), f32, dev), _dense("lengths", lengths, (B,), torch.int32, dev),
-            _dense("reset", reset, (T, B), f32, dev), _dense("state", state, ss, f32, dev), _dense("state_out", state_out, ss, f32, dev),
-            0, 0, 0, 0, 0, 0)
-    rest = (*sq, *sk, *sv, *so, *_ROWS0, *_ROWS0, *_ROWS0, *_ROWS0, T, B, H, dk, dv, dt, scale, 0)
+    sq, sk, sv, so = q.stride(), k.stride(), v.stride(), out.stride()
+    if not (q.get_device() == k.get_device() == v.get_device() == out.get_device() == log_decay.get_device() == dev and
+            k.dtype is v.dtype is out.dtype is typ and log_decay.dtype is f32 and k.shape == ks and v.shape == out.shape == vs and
+            log_decay.shape == (H,) and sq[3] == sk[3] == sv[3] == so[3] == 1 and log_decay.is_contiguous()):
+        _explain(dev, ("q", q, ks, typ, False), ("k", k, ks, typ, False), ("v", v, vs, typ, False), ("out", out, vs, typ, False),
+                 ("log_decay", log_decay, (H,), f32, True))
+    if not (lengths is reset is state is state_out is None):
+        _explain(dev, ("lengths", lengths, (B,), torch.int32, True), ("reset", reset, (T, B), f32, True), ("state", state, ss, f32, True),
+                 ("state_out", state_out, ss, f32, True))
+    ptrs = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), log_decay.data_ptr(), ptr(lengths) or 0, ptr(reset) or 0, ptr(state) or 0,
+            ptr(state_out) or 0, 0, 0, 0, 0, 0, 0)
+    rest = (*sq[:3], *sk[:3], *sv[:3], *so[:3], 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, T, B, H, dk, dv, dt, scale, 0)
     p = _LINATTN.pack(*ptrs, 0, 0, *rest)
     need = _lib.load().xrl_linattn_workspace_floats(p, 0)
     if need:
         ws = _workspace(workspace, need, dev)
         p = _LINATTN.pack(*ptrs, ws.data_ptr(), ws.numel(), *rest)
-    call("xrl_linattn_forward", p, stream_ptr())
+    call("xrl_linattn_forward", p, _raw_stream(dev))
 
 
 def linattn_backward(q, k, v, d_out, d_q, d_k, d_v, log_decay, scale=1.0, lengths=None, reset=None, state=None, d_state_out=None,
@@ -1322,23 +1314,25 @@ def linattn_backward(q, k, v, d_out, d_q, d_k, d_v, log_decay, scale=1.0, length
     per head, to be summed by the caller."""
     T, B, H, dk, dv, dt, dev = _linattn_sizes(q, v)
     f32, typ, ks, vs, ss = torch.float32, q.dtype, (T, B, H, dk), (T, B, H, dv), (B, H, dk, dv)
-    pq, sq = _rows("q", q, ks, typ, dev)
-    pk, sk = _rows("k", k, ks, typ, dev)
-    pv, sv = _rows("v", v, vs, typ, dev)
-    pdo, sdo = _rows("d_out", d_out, vs, typ, dev)
-    pdq, sdq = _rows("d_q", d_q, ks, typ, dev)
-    pdk, sdk = _rows("d_k", d_k, ks, typ, dev)
-    pdv, sdv = _rows("d_v", d_v, vs, typ, dev)
-    ptrs = (pq, pk, pv, 0, _dense("log_decay", log_decay, (H,), f32, dev), _dense("lengths", lengths, (B,), torch.int32, dev),
-            _dense("reset", reset, (T, B), f32, dev), _dense("state", state, ss, f32, dev), 0, pdo, pdq, pdk, pdv,
-            _dense("d_state_out", d_state_out, ss, f32, dev), _dense("d_state", d_state, ss, f32, dev))
-    rest = (*sq, *sk, *sv, *_ROWS0, *sdo, *sdq, *sdk, *sdv, T, B, H, dk, dv, dt, scale, 0)
+    sq, sk, sv, sdo, sdq, sdk, sdv = q.stride(), k.stride(), v.stride(), d_out.stride(), d_q.stride(), d_k.stride(), d_v.stride()
+    if not (q.get_device() == k.get_device() == v.get_device() == d_out.get_device() == d_q.get_device() == d_k.get_device() == d_v.get_device()
+            == log_decay.get_device() == dev and k.dtype is v.dtype is d_out.dtype is d_q.dtype is d_k.dtype is d_v.dtype is typ and
+            log_decay.dtype is f32 and k.shape == d_q.shape == d_k.shape == ks and v.shape == d_out.shape == d_v.shape == vs and log_decay.shape == (H,)
+            and sq[3] == sk[3] == sv[3] == sdo[3] == sdq[3] == sdk[3] == sdv[3] == 1 and log_decay.is_contiguous()):
+        _explain(dev, ("q", q, ks, typ, False), ("k", k, ks, typ, False), ("v", v, vs, typ, False), ("d_out", d_out, vs, typ, False),
+                 ("d_q", d_q, ks, typ, False), ("d_k", d_k, ks, typ, False), ("d_v", d_v, vs, typ, False), ("log_decay", log_decay, (H,), f32, True))
+    if not (lengths is reset is state is d_state_out is d_state is None):
+        _explain(dev, ("lengths", lengths, (B,), torch.int32, True), ("reset", reset, (T, B), f32, True), ("state", state, ss, f32, True),
+                 ("d_state_out", d_state_out, ss, f32, True), ("d_state", d_state, ss, f32, True))
+    ptrs = (q.data_ptr(), k.data_ptr(), v.data_ptr(), 0, log_decay.data_ptr(), ptr(lengths) or 0, ptr(reset) or 0, ptr(state) or 0, 0, d_out.data_ptr(),
+            d_q.data_ptr(), d_k.data_ptr(), d_v.data_ptr(), ptr(d_state_out) or 0, ptr(d_state) or 0)
+    rest = (*sq[:3], *sk[:3], *sv[:3], 0, 0, 0, *sdo[:3], *sdq[:3], *sdk[:3], *sdv[:3], T, B, H, dk, dv, dt, scale, 0)
     p = _LINATTN.pack(*ptrs, 0, 0, *rest)
     need = _lib.load().xrl_linattn_workspace_floats(p, 1)
     if need:
         ws = _workspace(workspace, need, dev)
         p = _LINATTN.pack(*ptrs, ws.data_ptr(), ws.numel(), *rest)
-    call("xrl_linattn_backward", p, stream_ptr())
+    call("xrl_linattn_backward", p, _raw_stream(dev))
 
 
 def linattn_step(q, k, v, out, log_decay, state, state_out=None, scale=1.0, reset=None):
@@ -1346,33 +1340,46 @@ def linattn_step(q, k, v, out, log_decay, state, state_out=None, scale=1.0, rese
     into state_out."""
     if q.dim() != 3 or v.dim() != 3:
         raise XrlError(f"q, k, v: [B, H, d] each, got {tuple(q.shape)}, {tuple(v.shape)}")
-    B, H, dk = q.shape
-    dv, dt, dev = v.shape[2], _io_dtype(q), torch.cuda.current_device()
-    f32, typ, ks, vs, ss = torch.float32, q.dtype, (B, H, dk), (B, H, dv), (B, H, dk, dv)
-    pq, sq = _rows("q", q, ks, typ, dev)
-    pk, sk = _rows("k", k, ks, typ, dev)
-    pv, sv = _rows("v", v, vs, typ, dev)
-    po, so = _rows("out", out, vs, typ, dev)
-    ps = _dense("state", state, ss, f32, dev)
-    pn = ps if state_out is None else _dense("state_out", state_out, ss, f32, dev)
-    p = _LINATTN.pack(pq, pk, pv, po, _dense("log_decay", log_decay, (H,), f32, dev), 0, _dense("reset", reset, (B,), f32, dev), ps, pn,
-                      0, 0, 0, 0, 0, 0, 0, 0, 0, *sq, 0, *sk, 0, *sv, 0, *so, *_ROWS0, *_ROWS0, *_ROWS0, *_ROWS0, 1, B, H, dk, dv, dt, scale, 0)
-    call("xrl_linattn_step", p, stream_ptr())
+    if state_out is None:
+        state_out = state
+    B, H, dk = ks = q.shape
+    vs, typ, f32, dev = v.shape, q.dtype, torch.float32, torch.cuda.current_device()
+    dv, dt, ss = vs[2], _io_dtype(q), (B, H, dk, vs[2])
+    sq, sk, sv, so = q.stride(), k.stride(), v.stride(), out.stride()
+    if not (q.get_device() == k.get_device() == v.get_device() == out.get_device() == log_decay.get_device() == state.get_device() == state_out.get_device()
+            == dev and k.dtype is v.dtype is out.dtype is typ and log_decay.dtype is state.dtype is state_out.dtype is f32 and k.shape == ks and
+            vs[0] == B and vs[1] == H and out.shape == vs and state.shape == state_out.shape == ss and log_decay.shape == (H,) and
+            sq[2] == sk[2] == sv[2] == so[2] == 1 and log_decay.is_contiguous() and state.is_contiguous() and state_out.is_contiguous()):
+        vs = (B, H, dv)
+        _explain(dev, ("q", q, ks, typ, False), ("k", k, ks, typ, False), ("v", v, vs, typ, False), ("out", out, vs, typ, False),
+                 ("log_decay", log_decay, (H,), f32, True), ("state", state, ss, f32, True), ("state_out", state_out, ss, f32, True))
+    if reset is not None:
+        _explain(dev, ("reset", reset, (B,), f32, True))
+    p = _LINATTN.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), log_decay.data_ptr(), 0, ptr(reset) or 0, state.data_ptr(),
+                      state_out.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, 0, sq[0], sq[1], 0, sk[0], sk[1], 0, sv[0], sv[1], 0, so[0], so[1],
+                      0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 1, B, H, dk, dv, dt, scale, 0)
+    call("xrl_linattn_step", p, _raw_stream(dev))
 
 
-def _norm_args(x, kind, gate_act, eps):
+def _norm_args(x, kind, gate_act, eps, rows, vectors):
+    """-> shape, type code, device; rows and vectors: (name, tensor) pairs, checked."""
     if x.dim() != 2:
         raise XrlError(f"x: [N, D], got {tuple(x.shape)}")
     if kind not in NORM_KIND or gate_act not in ACT or not eps > 0:
         raise XrlError(f"kind {kind!r} of {sorted(NORM_KIND)}, gate_act {gate_act!r} of the activations, eps {eps} > 0")
-    return x.shape, (x.shape[1],), x.dtype, _io_dtype(x), torch.cuda.current_device()
+    shape, typ, f32, dev = x.shape, x.dtype, torch.float32, torch.cuda.current_device()
+    vec = shape[1:]
+    for name, t in rows:
+        if t is not None and (t.get_device() != dev or t.dtype is not typ or t.shape != shape or t.stride()[1] != 1):
+            _explain(dev, (name, t, shape, typ, False))
+    for name, t in vectors:
+        if t is not None and (t.get_device() != dev or t.dtype is not f32 or t.shape != vec or not t.is_contiguous()):
+            _explain(dev, (name, t, vec, f32, True))
+    return shape, _io_dtype(x), dev
 
 
-def _opt_rows(name, t, shape, dtype, device):
-    if t is None:
-        return 0, 0
-    p, st = _rows(name, t, shape, dtype, device)
-    return p, st[0]
+def _ld(t):
+    return 0 if t is None else t.stride(0)
 
 
 def block_norm_forward(x, u, y, n=None, gate=None, gate_act="sigmoid", scale=None, w_post=None, b_post=None, w_pre=None, b_pre=None,
@@ -1381,18 +1388,12 @@ def block_norm_forward(x, u, y, n=None, gate=None, gate_act="sigmoid", scale=Non
         y = x + scale * act(gate) * (norm(u) * w_post + b_post),    n = norm(y) * w_pre + b_pre
     x (residual stream), u (output of the block), gate, y (stream after it), n (input of the next block): [N, D] float32 or bfloat16,
     D up to 8192, rows of any stride; scale, weights, biases [D] float32, a missing one is 1 or 0.  kind "rms" or "layer".  y may be x."""
-    shape, vec, typ, dt, dev = _norm_args(x, kind, gate_act, eps)
-    f32 = torch.float32
-    px, lx = _opt_rows("x", x, shape, typ, dev)
-    pu, lu = _opt_rows("u", u, shape, typ, dev)
-    pg, lg = _opt_rows("gate", gate, shape, typ, dev)
-    py, ly = _opt_rows("y", y, shape, typ, dev)
-    pn, ln = _opt_rows("n", n, shape, typ, dev)
-    p = _BLOCK_NORM.pack(px, pu, pg, py, pn, _dense("scale", scale, vec, f32, dev), _dense("w_post", w_post, vec, f32, dev),
-                         _dense("b_post", b_post, vec, f32, dev), _dense("w_pre", w_pre, vec, f32, dev), _dense("b_pre", b_pre, vec, f32, dev),
-                         0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, shape[0], lx, lu, lg, ly, ln, 0, 0, 0, 0, 0, shape[1], dt, NORM_KIND[kind],
-                         ACT[gate_act], eps, 0)
-    call("xrl_block_norm_forward", p, stream_ptr())
+    shape, dt, dev = _norm_args(x, kind, gate_act, eps, (("x", x), ("u", u), ("gate", gate), ("y", y), ("n", n)),
+                                (("scale", scale), ("w_post", w_post), ("b_post", b_post), ("w_pre", w_pre), ("b_pre", b_pre)))
+    p = _BLOCK_NORM.pack(x.data_ptr(), u.data_ptr(), ptr(gate) or 0, y.data_ptr(), ptr(n) or 0, ptr(scale) or 0, ptr(w_post) or 0, ptr(b_post) or 0,
+                         ptr(w_pre) or 0, ptr(b_pre) or 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, shape[0], x.stride(0), u.stride(0), _ld(gate), y.stride(0),
+                         _ld(n), 0, 0, 0, 0, 0, shape[1], dt, NORM_KIND[kind], ACT[gate_act], eps, 0)
+    call("xrl_block_norm_forward", p, _raw_stream(dev))
 
 
 def block_norm_workspace_floats(N, D, dtype=torch.float32):
@@ -1408,27 +1409,21 @@ def block_norm_backward(x, u, d_y, d_n, d_x, d_u, d_gate=None, d_scale=None, d_w
     """Gradients of block_norm_forward (xrl_block_norm_backward) from d_y and d_n (either may be None: 0): d_x, d_u, where given d_gate
     [N, D] and the sums over the rows d_scale, d_w_post, d_b_post, d_w_pre, d_b_pre [D] float32.  Needs x, u and gate of the forward pass,
     nothing else; the order of the sums is fixed.  d_x may be d_y."""
-    shape, vec, typ, dt, dev = _norm_args(x, kind, gate_act, eps)
-    f32 = torch.float32
-    px, lx = _opt_rows("x", x, shape, typ, dev)
-    pu, lu = _opt_rows("u", u, shape, typ, dev)
-    pg, lg = _opt_rows("gate", gate, shape, typ, dev)
-    pdy, ldy = _opt_rows("d_y", d_y, shape, typ, dev)
-    pdn, ldn = _opt_rows("d_n", d_n, shape, typ, dev)
-    pdx, ldx = _opt_rows("d_x", d_x, shape, typ, dev)
-    pdu, ldu = _opt_rows("d_u", d_u, shape, typ, dev)
-    pdg, ldg = _opt_rows("d_gate", d_gate, shape, typ, dev)
-    ptrs = (px, pu, pg, 0, 0, _dense("scale", scale, vec, f32, dev), _dense("w_post", w_post, vec, f32, dev), _dense("b_post", b_post, vec, f32, dev),
-            _dense("w_pre", w_pre, vec, f32, dev), _dense("b_pre", b_pre, vec, f32, dev), pdy, pdn, pdx, pdu, pdg,
-            _dense("d_scale", d_scale, vec, f32, dev), _dense("d_w_post", d_w_post, vec, f32, dev), _dense("d_b_post", d_b_post, vec, f32, dev),
-            _dense("d_w_pre", d_w_pre, vec, f32, dev), _dense("d_b_pre", d_b_pre, vec, f32, dev))
-    rest = (shape[0], lx, lu, lg, 0, 0, ldy, ldn, ldx, ldu, ldg, shape[1], dt, NORM_KIND[kind], ACT[gate_act], eps, 0)
+    shape, dt, dev = _norm_args(x, kind, gate_act, eps,
+                                (("x", x), ("u", u), ("gate", gate), ("d_y", d_y), ("d_n", d_n), ("d_x", d_x), ("d_u", d_u), ("d_gate", d_gate)),
+                                (("scale", scale), ("w_post", w_post), ("b_post", b_post), ("w_pre", w_pre), ("b_pre", b_pre), ("d_scale", d_scale),
+                                 ("d_w_post", d_w_post), ("d_b_post", d_b_post), ("d_w_pre", d_w_pre), ("d_b_pre", d_b_pre)))
+    ptrs = (x.data_ptr(), u.data_ptr(), ptr(gate) or 0, 0, 0, ptr(scale) or 0, ptr(w_post) or 0, ptr(b_post) or 0, ptr(w_pre) or 0, ptr(b_pre) or 0,
+            ptr(d_y) or 0, ptr(d_n) or 0, d_x.data_ptr(), d_u.data_ptr(), ptr(d_gate) or 0, ptr(d_scale) or 0, ptr(d_w_post) or 0, ptr(d_b_post) or 0,
+            ptr(d_w_pre) or 0, ptr(d_b_pre) or 0)
+    rest = (shape[0], x.stride(0), u.stride(0), _ld(gate), 0, 0, _ld(d_y), _ld(d_n), d_x.stride(0), d_u.stride(0), _ld(d_gate), shape[1], dt,
+            NORM_KIND[kind], ACT[gate_act], eps, 0)
     need = _lib.load().xrl_block_norm_workspace_floats(_BLOCK_NORM.pack(*ptrs, 0, 0, *rest))
     ws = (0, 0)
     if need:
         buf = _workspace(workspace, need, dev)
         ws = (buf.data_ptr(), buf.numel())
-    call("xrl_block_norm_backward", _BLOCK_NORM.pack(*ptrs, *ws, *rest), stream_ptr())
+    call("xrl_block_norm_backward", _BLOCK_NORM.pack(*ptrs, *ws, *rest), _raw_stream(dev))
 
 
 def distill_loss(logits, teacher_idx, teacher_logits, loss, d_logits=None, avail=None, weight=None, temperature=1.0, grad_scale=1.0):
@@ -1440,15 +1435,22 @@ def distill_loss(logits, teacher_idx, teacher_logits, loss, d_logits=None, avail
     valid teacher entry, without an available logit or of weight 0 has loss 0 and gradient 0."""
     if logits.dim() != 2 or teacher_idx.dim() != 2:
         raise XrlError("logits: [N, A], teacher_idx: [N, K]")
-    dev, typ, f32 = torch.cuda.current_device(), logits.dtype, torch.float32
-    shape = N, A = logits.shape
+    dev, typ, f32, i32 = torch.cuda.current_device(), logits.dtype, torch.float32, torch.int32
+    N, A = shape = logits.shape
     K = teacher_idx.shape[1]
-    ps, ld = _opt_rows("logits", logits, shape, typ, dev)
-    pd, ldd = _opt_rows("d_logits", d_logits, shape, typ, dev)
-    p = _DISTILL.pack(ps, _dense("teacher_idx", teacher_idx, (N, K), torch.int32, dev), _dense("teacher_logits", teacher_logits, (N, K), typ, dev),
-                      _dense("avail", avail, shape, f32, dev), _dense("weight", weight, (N,), f32, dev), _dense("loss", loss, (N,), f32, dev), pd,
-                      N, ld, ldd, A, K, _io_dtype(logits), temperature, grad_scale, 0)
-    call("xrl_distill_loss", p, stream_ptr())
+    top = (N, K)
+    if not (logits.get_device() == teacher_idx.get_device() == teacher_logits.get_device() == loss.get_device() == dev and teacher_idx.dtype is i32 and
+            teacher_logits.dtype is typ and loss.dtype is f32 and teacher_idx.shape == teacher_logits.shape == top and loss.shape == (N,) and
+            logits.stride()[1] == 1 and teacher_idx.is_contiguous() and teacher_logits.is_contiguous() and loss.is_contiguous()):
+        _explain(dev, ("logits", logits, shape, typ, False), ("teacher_idx", teacher_idx, top, i32, True), ("teacher_logits", teacher_logits, top, typ, True),
+                 ("loss", loss, (N,), f32, True))
+    if d_logits is not None and (d_logits.get_device() != dev or d_logits.dtype is not typ or d_logits.shape != shape or d_logits.stride()[1] != 1):
+        _explain(dev, ("d_logits", d_logits, shape, typ, False))
+    if not (avail is weight is None):
+        _explain(dev, ("avail", avail, shape, f32, True), ("weight", weight, (N,), f32, True))
+    p = _DISTILL.pack(logits.data_ptr(), teacher_idx.data_ptr(), teacher_logits.data_ptr(), ptr(avail) or 0, ptr(weight) or 0, loss.data_ptr(),
+                      ptr(d_logits) or 0, N, logits.stride(0), _ld(d_logits), A, K, _io_dtype(logits), temperature, grad_scale, 0)
+    call("xrl_distill_loss", p, _raw_stream(dev))
 
 
 def sync_target(params, target, P, state, sync_frequency):
