@@ -4,10 +4,13 @@
 //
 // Bound by memory: forward 3 reads + 2 writes, backward 5 reads + 3 writes of N x D values and nothing saved in between -- the backward
 // pass recomputes p, y and both statistics from the x, u and gate it needs anyway.  A row lives in the registers of L lanes, 8 values
-// each, from its one load to its one store; the parameters and the gradient sums over the rows stay in registers over all rows of a
-// workgroup.  Those sums leave as one line of partials per workgroup and a second launch adds the lines in a fixed order (no atomics).
+// each, from its one load to its one store; the gradient sums over the rows stay in registers over all rows of a workgroup, the parameters in LDS.
+// Those sums leave as one line of partials per workgroup and a second launch adds the lines in a fixed order (no atomics).
+// Measured, forward and backward: 65536 x 256 f32 with a gate, rms 65 us (5.2 TB/s) and 103 us (5.2), as a copy; 30011 x 2048 bf16, layer, 142 us
+// (4.3) and 240 us (4.1): a row of 2048 is four waves that meet six times, and the vector instructions of two or three rows a CU do not hide that.
 #include "args.h"
 #include "io16.h"
+#include "lanes.h"
 
 namespace xrl {
 
@@ -23,8 +26,12 @@ __device__ __forceinline__ float gate_act_c(float z) {
     if (ACT == XRL_ACT_SIGMOID) return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * z));
     return act_apply_c<ACT>(z);
 }
-constexpr int NORM_SUMS = 5;           // d_scale, d_w_post, d_b_post, d_w_pre, d_b_pre
+// Sums over the rows, with a the activated gate, uhat and yhat the normalised u and y:  S0 = sum a d_y,  S1 = sum a d_y uhat,  S2 = sum d_n yhat,
+// S3 = sum d_n.  They give d_scale = w_post S1 + b_post S0, d_w_post = scale S1, d_b_post = scale S0, d_w_pre = S2, d_b_pre = S3.  (Where w_post uhat
+// and b_post cancel in p, d_scale loses no more than the rounding of uhat costs it anyway.)
+constexpr int NORM_SUMS = 4;
 
+// FULL below: rows of exactly 8 L values, without the checks of a row's end (30011 x 2048 bf16: with the sums by lanes.h 431 -> 386 us)
 template <int L>
 struct norm_geom {
     static constexpr int THREADS = L < 256 ? (L > 64 ? L : 256) : L;
@@ -33,7 +40,7 @@ struct norm_geom {
 };
 
 // eight neighbouring values of a row as they are stored; absent ones 0
-template <typename E>
+template <typename E, bool FULL>
 struct row8 {
     static constexpr int PER = row16<E>::PER, N = NV / PER;
     u32x4_t v[N];
@@ -41,10 +48,10 @@ struct row8 {
         typedef row16<E> R;
 #pragma unroll
         for (int q = 0; q < N; ++q) { const u32x4_t zero = {0, 0, 0, 0}; v[q] = zero; }
-        if (at + NV <= D) {
+        if (FULL ? D > 0 : at + NV <= D) {
 #pragma unroll
             for (int q = 0; q < N; ++q) v[q] = R::load(row + at + PER * q);
-        } else if (at < D) {
+        } else if (!FULL && at < D) {
 #pragma unroll
             for (int m = 0; m < NV; ++m)
                 if (at + m < D) R::put(v[m / PER], m % PER, R::bits(row + at + m));
@@ -56,7 +63,7 @@ struct row8 {
     }
     static __device__ __forceinline__ void store(E* row, int at, int D, const float (&f)[NV]) {
         typedef row16<E> R;
-        if (at + NV <= D) {
+        if (FULL || at + NV <= D) {
 #pragma unroll
             for (int q = 0; q < N; ++q) R::store(row + at + PER * q, R::pack(f + PER * q));
         } else if (at < D) {
@@ -67,10 +74,32 @@ struct row8 {
     }
 };
 
-__device__ __forceinline__ void norm_param(const float* p, int at, int D, float missing, float (&v)[NV]) {
+// A row's parameters in LDS, 16 bytes a lane and read: kept in registers they would cost 8 each and with them every third or second wave.
+template <int L>
+struct norm_params {
+    f32x4_t (*lds)[2][L];                                            // [parameter][half][lane]
+    __device__ __forceinline__ void fill(int which, const float* p, float missing, int D) {
+        for (int c = threadIdx.x; c < 2 * L; c += norm_geom<L>::THREADS) {
+            const int half = c / L, l = c % L;
+            f32x4_t v;
 #pragma unroll
-    for (int m = 0; m < NV; ++m) v[m] = at + m < D ? (p ? p[at + m] : missing) : 0.f;
-}
+            for (int i = 0; i < 4; ++i) {
+                const int e = l * NV + 4 * half + i;
+                v[i] = e < D ? (p ? p[e] : missing) : 0.f;
+            }
+            lds[which][half][l] = v;
+        }
+    }
+    __device__ __forceinline__ void get(int which, int lane, float (&v)[NV]) const {
+        asm volatile("" : "+v"(lane));                               // read again for every use
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const f32x4_t q = lds[which][half][lane];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[4 * half + i] = q[i];
+        }
+    }
+};
 
 // Sums over the L lanes of a row.  Across waves through LDS with one barrier: consecutive sums use other slots of `scratch`, and a slot
 // comes round again only two barriers later.
@@ -79,8 +108,8 @@ struct row_sum_t {
     float2 (*scratch)[16];
     int slot;
     __device__ __forceinline__ float2 operator()(float a, float b) {
-#pragma unroll
-        for (int off = (L < 64 ? L : 64) / 2; off > 0; off >>= 1) { a += __shfl_xor(a, off, 64); b += __shfl_xor(b, off, 64); }
+        a = lane_sum<L < 64 ? L : 64>(a);
+        b = lane_sum<L < 64 ? L : 64>(b);
         if (L > 64) {
             const int w = threadIdx.x >> 6;
             slot = slot == 2 ? 0 : slot + 1;
@@ -93,8 +122,7 @@ struct row_sum_t {
         return make_float2(a, b);
     }
     __device__ __forceinline__ float operator()(float a) {
-#pragma unroll
-        for (int off = (L < 64 ? L : 64) / 2; off > 0; off >>= 1) a += __shfl_xor(a, off, 64);
+        a = lane_sum<L < 64 ? L : 64>(a);
         if (L > 64) {
             const int w = threadIdx.x >> 6;
             slot = slot == 2 ? 0 : slot + 1;
@@ -109,7 +137,7 @@ struct row_sum_t {
 };
 
 // v := (v - mean) r (layer) or v r; returns r.  The variance is taken of the centred values (no difference of large sums).
-template <int L, bool LN>
+template <int L, bool LN, bool FULL>
 __device__ __forceinline__ float normalize(float (&v)[NV], int at, int D, float inv_d, float eps, row_sum_t<L>& sum) {
     if (LN) {
         float s = 0.f;
@@ -117,7 +145,7 @@ __device__ __forceinline__ float normalize(float (&v)[NV], int at, int D, float 
         for (int m = 0; m < NV; ++m) s += v[m];
         const float mean = sum(s) * inv_d;
 #pragma unroll
-        for (int m = 0; m < NV; ++m) v[m] = at + m < D ? v[m] - mean : 0.f;
+        for (int m = 0; m < NV; ++m) v[m] = FULL || at + m < D ? v[m] - mean : 0.f;
     }
     float q = 0.f;
 #pragma unroll
@@ -128,58 +156,68 @@ __device__ __forceinline__ float normalize(float (&v)[NV], int at, int D, float 
     return r;
 }
 
-template <typename E, int L, bool LN>
+template <typename E, int L, bool LN, bool FULL>
 __global__ void __launch_bounds__(norm_geom<L>::THREADS) block_norm_fwd_kernel(xrl_block_norm_t p) {
     using G = norm_geom<L>;
     __shared__ float2 scratch[3][16];
     row_sum_t<L> sum{scratch, 0};
     const int lane = threadIdx.x % L, at = lane * NV, D = p.D;
     const float inv_d = 1.f / (float)D;
-    float sc[NV], w0[NV], b0[NV], w1[NV], b1[NV];
-    norm_param(p.scale, at, D, 1.f, sc);
-    norm_param(p.w_post, at, D, 1.f, w0);
-    norm_param(p.b_post, at, D, 0.f, b0);
-    norm_param(p.w_pre, at, D, 1.f, w1);
-    norm_param(p.b_pre, at, D, 0.f, b1);
-    row8<E> rx, ru, rg;
+    __shared__ f32x4_t pars[3][2][L];                                // the shifts in registers: five here, 40 KB for 2048 values, leave room for three waves
+    norm_params<L> par{pars};
+    par.fill(0, p.scale, 1.f, D); par.fill(1, p.w_post, 1.f, D); par.fill(2, p.w_pre, 1.f, D);
+    float b0[NV], b1[NV];
+#pragma unroll
+    for (int m = 0; m < NV; ++m) {
+        b0[m] = p.b_post && at + m < D ? p.b_post[at + m] : 0.f;
+        b1[m] = p.b_pre && at + m < D ? p.b_pre[at + m] : 0.f;
+    }
+    __syncthreads();
+    row8<E, FULL> rx, ru, rg;
     auto request = [&](int64_t row) {
         const int width = row < p.N ? D : 0;
         ru.load((const E*)p.u + row * p.ld_u, at, width);
         rx.load((const E*)p.x + row * p.ld_x, at, width);
         if (p.gate) rg.load((const E*)p.gate + row * p.ld_gate, at, width);
     };
-    constexpr bool AHEAD = L < 1024;                                 // 1024 threads leave no registers for it
+    constexpr bool AHEAD = L < 1024;                                 // 1024 threads leave no registers for it; both passes of 2048 bf16: 471 -> 431 us
     if (AHEAD) request((int64_t)blockIdx.x * G::ROWS + threadIdx.x / L);
     const int64_t step = (int64_t)gridDim.x * G::ROWS;
     for (int64_t base = (int64_t)blockIdx.x * G::ROWS; base < p.N; base += step) {       // whole workgroups go round: barriers inside
         const int64_t row = base + threadIdx.x / L;
         const bool live = row < p.N;
-        float x[NV], u[NV], g[NV] = {};
+        float x[NV], u[NV], g[NV];
         if (!AHEAD) request(row);
         ru.get(u); rx.get(x);
         if (p.gate) rg.get(g);
         if (AHEAD && base + step < p.N) request(row + step);         // the next row is on its way while this one is worked on
-        normalize<L, LN>(u, at, D, inv_d, p.eps, sum);
+        normalize<L, LN, FULL>(u, at, D, inv_d, p.eps, sum);
         if (p.gate) {
             XRL_ACT_DISPATCH(p.gate_act, _Pragma("unroll") for (int m = 0; m < NV; ++m) g[m] = gate_act_c<ACT>(g[m]);)
-        }
+        } else {
 #pragma unroll
-        for (int m = 0; m < NV; ++m) {
-            const float b = fma_f(u[m], w0[m], b0[m]);
-            x[m] = fma_f(p.gate ? g[m] * sc[m] : sc[m], b, x[m]);
+            for (int m = 0; m < NV; ++m) g[m] = 1.f;
         }
-        if (live) row8<E>::store((E*)p.y + row * p.ld_y, at, D, x);
+        float w[NV];
+        par.get(1, lane, w);
+#pragma unroll
+        for (int m = 0; m < NV; ++m) u[m] = fma_f(u[m], w[m], b0[m]);
+        par.get(0, lane, w);
+#pragma unroll
+        for (int m = 0; m < NV; ++m) x[m] = fma_f(g[m] * w[m], u[m], x[m]);
+        if (live) row8<E, FULL>::store((E*)p.y + row * p.ld_y, at, D, x);
         if (p.n) {
-            normalize<L, LN>(x, at, D, inv_d, p.eps, sum);
+            normalize<L, LN, FULL>(x, at, D, inv_d, p.eps, sum);
+            par.get(2, lane, w);
 #pragma unroll
-            for (int m = 0; m < NV; ++m) x[m] = fma_f(x[m], w1[m], b1[m]);
-            if (live) row8<E>::store((E*)p.n + row * p.ld_n, at, D, x);
+            for (int m = 0; m < NV; ++m) x[m] = fma_f(x[m], w[m], b1[m]);
+            if (live) row8<E, FULL>::store((E*)p.n + row * p.ld_n, at, D, x);
         }
     }
 }
 
 // d := r (d - xhat mean(d xhat) [- mean(d)]): gradient through the normalisation
-template <int L, bool LN>
+template <int L, bool LN, bool FULL>
 __device__ __forceinline__ void normalize_back(float (&d)[NV], const float (&xhat)[NV], float r, int at, int D, float inv_d,
                                                row_sum_t<L>& sum) {
     float a = 0.f, b = 0.f;
@@ -188,25 +226,24 @@ __device__ __forceinline__ void normalize_back(float (&d)[NV], const float (&xha
     if (LN) { const float2 t = sum(a, b); a = t.x * inv_d; b = t.y * inv_d; }
     else a = sum(a) * inv_d;
 #pragma unroll
-    for (int m = 0; m < NV; ++m) d[m] = at + m < D ? r * fma_f(-xhat[m], a, LN ? d[m] - b : d[m]) : 0.f;
+    for (int m = 0; m < NV; ++m) d[m] = FULL || at + m < D ? r * fma_f(-xhat[m], a, LN ? d[m] - b : d[m]) : 0.f;
 }
 
-template <typename E, int L, bool LN>
+template <typename E, int L, bool LN, bool FULL>
 __global__ void __launch_bounds__(norm_geom<L>::THREADS) block_norm_bwd_kernel(xrl_block_norm_t p) {
     using G = norm_geom<L>;
     __shared__ float2 scratch[3][16];
     row_sum_t<L> sum{scratch, 0};
     const int lane = threadIdx.x % L, at = lane * NV, D = p.D;
     const float inv_d = 1.f / (float)D;
-    float sc[NV], w0[NV], b0[NV], w1[NV];
-    norm_param(p.scale, at, D, 1.f, sc);
-    norm_param(p.w_post, at, D, 1.f, w0);
-    norm_param(p.b_post, at, D, 0.f, b0);
-    norm_param(p.w_pre, at, D, 1.f, w1);
+    __shared__ f32x4_t pars[4][2][L];
+    norm_params<L> par{pars};
+    par.fill(0, p.scale, 1.f, D); par.fill(1, p.w_post, 1.f, D); par.fill(2, p.b_post, 0.f, D); par.fill(3, p.w_pre, 1.f, D);
+    __syncthreads();
     float acc[NORM_SUMS][NV] = {};
     // the next row is on its way while this one is worked on; 1024 threads leave no registers for that
     constexpr bool AHEAD = L < 1024;
-    row8<E> rx, ru_, rg, ry_, rn;
+    row8<E, FULL> rx, ru_, rg, ry_, rn;
     auto request = [&](int64_t row) {
         const int width = row < p.N ? D : 0;
         ru_.load((const E*)p.u + row * p.ld_u, at, width);
@@ -220,47 +257,53 @@ __global__ void __launch_bounds__(norm_geom<L>::THREADS) block_norm_bwd_kernel(x
     for (int64_t base = (int64_t)blockIdx.x * G::ROWS; base < p.N; base += step) {
         const int64_t row = base + threadIdx.x / L;
         const bool live = row < p.N;
-        float x[NV], u[NV], g[NV] = {}, dy[NV] = {}, dn[NV] = {}, t[NV];
+        float x[NV], u[NV], g[NV], dy[NV] = {}, dn[NV] = {}, t[NV];
         if (!AHEAD) request(row);
         ru_.get(u); rx.get(x);
         if (p.gate) rg.get(g);
         if (p.d_y) ry_.get(dy);
         if (p.d_n) rn.get(dn);
         if (AHEAD && base + step < p.N) request(row + step);
-        const float ru = normalize<L, LN>(u, at, D, inv_d, p.eps, sum);
+        const float ru = normalize<L, LN, FULL>(u, at, D, inv_d, p.eps, sum);
         if (p.gate) {
             XRL_ACT_DISPATCH(p.gate_act, _Pragma("unroll") for (int m = 0; m < NV; ++m) g[m] = gate_act_c<ACT>(g[m]);)
+        } else {
+#pragma unroll
+            for (int m = 0; m < NV; ++m) g[m] = 1.f;
         }
-        float pm[NV];                                                // the normed block before gate and scale
+        float w[NV], sc[NV], pm[NV];                                 // pm: the block's part before gate and scale
+        par.get(1, lane, w); par.get(2, lane, pm);
 #pragma unroll
-        for (int m = 0; m < NV; ++m) pm[m] = fma_f(u[m], w0[m], b0[m]);
+        for (int m = 0; m < NV; ++m) pm[m] = fma_f(u[m], w[m], pm[m]);
         if (p.d_n) {
+            par.get(0, lane, sc);
 #pragma unroll
-            for (int m = 0; m < NV; ++m) x[m] = fma_f(p.gate ? g[m] * sc[m] : sc[m], pm[m], x[m]);
-            const float ry = normalize<L, LN>(x, at, D, inv_d, p.eps, sum);
+            for (int m = 0; m < NV; ++m) x[m] = fma_f(g[m] * sc[m], pm[m], x[m]);
+            const float ry = normalize<L, LN, FULL>(x, at, D, inv_d, p.eps, sum);
+            par.get(3, lane, w);
 #pragma unroll
-            for (int m = 0; m < NV; ++m) { acc[3][m] = fma_f(dn[m], x[m], acc[3][m]); acc[4][m] += dn[m]; t[m] = dn[m] * w1[m]; }
-            normalize_back<L, LN>(t, x, ry, at, D, inv_d, sum);
+            for (int m = 0; m < NV; ++m) { acc[2][m] = fma_f(dn[m], x[m], acc[2][m]); acc[3][m] += dn[m]; t[m] = dn[m] * w[m]; }
+            normalize_back<L, LN, FULL>(t, x, ry, at, D, inv_d, sum);
 #pragma unroll
             for (int m = 0; m < NV; ++m) dy[m] += t[m];
         }
-        if (live) row8<E>::store((E*)p.d_x + row * p.ld_d_x, at, D, dy);
+        if (live) row8<E, FULL>::store((E*)p.d_x + row * p.ld_d_x, at, D, dy);
         // y = x + scale a p: with a the activated gate
+        par.get(0, lane, sc); par.get(1, lane, w);
 #pragma unroll
         for (int m = 0; m < NV; ++m) {
-            const float da = p.gate ? dy[m] * g[m] : dy[m], dp = da * sc[m];
-            acc[0][m] = fma_f(da, pm[m], acc[0][m]);
-            acc[1][m] = fma_f(dp, u[m], acc[1][m]);
-            acc[2][m] += dp;
-            t[m] = dp * w0[m];
+            const float da = dy[m] * g[m];
+            acc[0][m] += da;
+            acc[1][m] = fma_f(da, u[m], acc[1][m]);
+            t[m] = da * sc[m] * w[m];
             dy[m] *= sc[m] * pm[m];                                  // gradient of the activated gate
         }
         if (p.d_gate) {
             XRL_ACT_DISPATCH(p.gate_act, _Pragma("unroll") for (int m = 0; m < NV; ++m) g[m] = dy[m] * act_grad_c<ACT>(g[m]);)
-            if (live) row8<E>::store((E*)p.d_gate + row * p.ld_d_gate, at, D, g);
+            if (live) row8<E, FULL>::store((E*)p.d_gate + row * p.ld_d_gate, at, D, g);
         }
-        normalize_back<L, LN>(t, u, ru, at, D, inv_d, sum);
-        if (live) row8<E>::store((E*)p.d_u + row * p.ld_d_u, at, D, t);
+        normalize_back<L, LN, FULL>(t, u, ru, at, D, inv_d, sum);
+        if (live) row8<E, FULL>::store((E*)p.d_u + row * p.ld_d_u, at, D, t);
     }
     // partial sums: over the rows of a wave, then over the waves (in wave order), one line per workgroup
     float* line = p.workspace + (size_t)blockIdx.x * NORM_SUMS * D;
@@ -295,23 +338,33 @@ __global__ void __launch_bounds__(norm_geom<L>::THREADS) block_norm_bwd_kernel(x
     }
 }
 
-// out[s][e] = sum of the workgroups' lines, 64 groups of lines a column, met in a fixed order
+// The sums of the workgroups' lines, 64 groups of lines a column, met in a fixed order, and what they give.  A workgroup has 16 columns of S0 and S1
+// or of S2 and S3.
 __global__ void __launch_bounds__(1024) block_norm_sums_kernel(xrl_block_norm_t p, int lines) {
-    __shared__ float part[64][17];
-    const int c = threadIdx.x & 15, r = threadIdx.x >> 4, width = NORM_SUMS * p.D;
-    const int col = blockIdx.x * 16 + c;
-    float t = 0.f;
-    if (col < width)
-        for (int i = r; i < lines; i += 64) t += p.workspace[(size_t)i * width + col];
-    part[r][c] = t;
+    __shared__ float part[2][64][17];
+    const int c = threadIdx.x & 15, r = threadIdx.x >> 4, width = NORM_SUMS * p.D, e = blockIdx.x * 16 + c;
+    const float* first = p.workspace + (size_t)blockIdx.y * 2 * p.D + e;
+    float s = 0.f, t = 0.f;
+    if (e < p.D)
+        for (int i = r; i < lines; i += 64) {
+            s += first[(size_t)i * width];
+            t += first[(size_t)i * width + p.D];
+        }
+    part[0][r][c] = s;
+    part[1][r][c] = t;
     __syncthreads();
-    if (threadIdx.x < 16 && col < width) {
-        float a = 0.f;
-        for (int i = 0; i < 64; ++i) a += part[i][c];
-        float* outs[NORM_SUMS] = {p.d_scale, p.d_w_post, p.d_b_post, p.d_w_pre, p.d_b_pre};
-#pragma unroll
-        for (int s = 0; s < NORM_SUMS; ++s)
-            if (outs[s] && col / p.D == s) outs[s][col % p.D] = a;
+    if (threadIdx.x < 16 && e < p.D) {
+        s = t = 0.f;
+        for (int i = 0; i < 64; ++i) { s += part[0][i][c]; t += part[1][i][c]; }
+        if (blockIdx.y == 0) {
+            const float sc = p.scale ? p.scale[e] : 1.f;
+            if (p.d_scale) p.d_scale[e] = fma_f(p.w_post ? p.w_post[e] : 1.f, t, p.b_post ? p.b_post[e] * s : 0.f);
+            if (p.d_w_post) p.d_w_post[e] = sc * t;
+            if (p.d_b_post) p.d_b_post[e] = sc * s;
+        } else {
+            if (p.d_w_pre) p.d_w_pre[e] = s;
+            if (p.d_b_pre) p.d_b_pre[e] = t;
+        }
     }
 }
 
@@ -321,10 +374,10 @@ static int norm_lanes(int D) {
     return L;
 }
 
-// workgroups of the backward pass: enough to fill the chip twice over, each with rows to keep its parameters and sums for
+// workgroups of the backward pass: as many as the registers let the chip hold (of 256 threads two a CU in f32, three in bf16), each with its rows
 static int norm_lines(const xrl_block_norm_t& p) {
     const int L = norm_lanes(p.D), threads = L < 256 ? (L > 64 ? L : 256) : L, rows = L > 64 ? 1 : threads / L;
-    const int64_t most = 512 * 256 / threads, need = (p.N + rows - 1) / rows;
+    const int64_t most = threads > 256 ? 256 : (p.dtype == XRL_F32 ? 512 : 768) * 256 / threads, need = (p.N + rows - 1) / rows;
     return (int)(need < most ? need : most);
 }
 
@@ -356,16 +409,16 @@ static int check_norm_tensors(const xrl_block_norm_t& p, bool backward) {
     return check_args(a, 19, pairs, 1);
 }
 
-template <typename E, bool LN>
+template <typename E, bool LN, bool FULL>
 static void launch_norm(const xrl_block_norm_t& p, bool backward, hipStream_t s) {
     const int L = norm_lanes(p.D);
 #define NORM_CASE(LL)                                                                                                            \
     case LL: {                                                                                                                   \
         using G = norm_geom<LL>;                                                                                                 \
-        if (backward) hipLaunchKernelGGL((block_norm_bwd_kernel<E, LL, LN>), dim3(norm_lines(p)), dim3(G::THREADS), 0, s, p); \
+        if (backward) hipLaunchKernelGGL((block_norm_bwd_kernel<E, LL, LN, FULL>), dim3(norm_lines(p)), dim3(G::THREADS), 0, s, p); \
         else {                                                                                                                   \
             const int64_t need = (p.N + G::ROWS - 1) / G::ROWS, most = 1024 * 256 / G::THREADS;                                  \
-            hipLaunchKernelGGL((block_norm_fwd_kernel<E, LL, LN>), dim3((int)(need < most ? need : most)), dim3(G::THREADS), 0, s, p); \
+            hipLaunchKernelGGL((block_norm_fwd_kernel<E, LL, LN, FULL>), dim3((int)(need < most ? need : most)), dim3(G::THREADS), 0, s, p); \
         }                                                                                                                        \
     } break;
     switch (L) { NORM_CASE(8) NORM_CASE(16) NORM_CASE(32) NORM_CASE(64) NORM_CASE(128) NORM_CASE(256) NORM_CASE(512) NORM_CASE(1024) }
@@ -374,8 +427,11 @@ static void launch_norm(const xrl_block_norm_t& p, bool backward, hipStream_t s)
 
 static int run_norm(const xrl_block_norm_t& p, bool backward, hipStream_t s) {
     const bool ln = p.kind == XRL_NORM_LAYER;
-    if (p.dtype == XRL_F32) { if (ln) launch_norm<float, true>(p, backward, s); else launch_norm<float, false>(p, backward, s); }
-    else { if (ln) launch_norm<bf16_t, true>(p, backward, s); else launch_norm<bf16_t, false>(p, backward, s); }
+    const bool full = p.D == norm_lanes(p.D) * NV;
+#define NORM_RUN(E, LN) do { if (full) launch_norm<E, LN, true>(p, backward, s); else launch_norm<E, LN, false>(p, backward, s); } while (0)
+    if (p.dtype == XRL_F32) { if (ln) NORM_RUN(float, true); else NORM_RUN(float, false); }
+    else { if (ln) NORM_RUN(bf16_t, true); else NORM_RUN(bf16_t, false); }
+#undef NORM_RUN
     XRL_CHECK_LAUNCH();
     return XRL_OK;
 }
@@ -410,7 +466,7 @@ extern "C" int xrl_block_norm_backward(const xrl_block_norm_t* pp, xrl_stream_t 
     if (p.N > 0)
         if (int rc = run_norm(p, true, as_stream(stream))) return rc;
     if (p.d_scale || p.d_w_post || p.d_b_post || p.d_w_pre || p.d_b_pre) {
-        hipLaunchKernelGGL(block_norm_sums_kernel, dim3((NORM_SUMS * p.D + 15) / 16), dim3(1024), 0, as_stream(stream), p, norm_lines(p));
+        hipLaunchKernelGGL(block_norm_sums_kernel, dim3((p.D + 15) / 16, 2), dim3(1024), 0, as_stream(stream), p, norm_lines(p));
         XRL_CHECK_LAUNCH();
     }
     return XRL_OK;

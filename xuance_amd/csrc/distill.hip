@@ -11,6 +11,7 @@
 // this size reaches 5.4), 33554 x 1000 bf16 42 us (3.2: the work on the entries shows), 256 x 18 9.7 us (the call and its launch).
 #include "args.h"
 #include "io16.h"
+#include "lanes.h"
 
 namespace xrl {
 
@@ -63,9 +64,6 @@ __device__ __forceinline__ int distill_entry(int i, float& t, const E* s, const 
     if (i < 0) t = -INFINITY;
     return i;
 }
-// a NaN has to reach the result, which fmaxf would pass over
-__device__ __forceinline__ float nan_max(float a, float b) { return __builtin_elementwise_maximum(a, b); }
-
 __device__ __forceinline__ void wave_lds_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); __builtin_amdgcn_wave_barrier(); }
 
 // Rows of up to 8 L actions: L lanes a row, 8 neighbouring actions a lane, no barrier.  LDS of a row: its entries (action, weight, policy's logit) and
@@ -82,16 +80,6 @@ __global__ void __launch_bounds__(256) distill_lanes_kernel(xrl_distill_t p) {
     float* tz = tq + ROWS * K;
     const int64_t row = (int64_t)blockIdx.x * ROWS + slot;
     if (row >= p.N) return;
-    auto sum = [&](float v) {
-#pragma unroll
-        for (int off = L / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-        return v;
-    };
-    auto top = [&](float v) {
-#pragma unroll
-        for (int off = L / 2; off > 0; off >>= 1) v = nan_max(v, __shfl_xor(v, off, 64));
-        return v;
-    };
     const float w = p.weight ? p.weight[row] : 1.f, kt = LOG2E / p.temperature, inv_tau = 1.f / p.temperature;
     const E* s = (const E*)p.logits + row * p.ld;
     const float* av = p.avail ? p.avail + row * A : nullptr;
@@ -111,7 +99,7 @@ __global__ void __launch_bounds__(256) distill_lanes_kernel(xrl_distill_t p) {
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) { m = nan_max(m, R::get(v[j / PER], j % PER)); at_action[8 * lane + j] = 0x7fffffff; }
-    tm = top(tm); m = top(m);
+    tm = lane_max<L>(tm); m = lane_max<L>(m);
     float any = 0.f, ts = 0.f, z = 0.f;
     wave_lds_fence();
     for (int k = lane; k < K; k += L)
@@ -125,7 +113,7 @@ __global__ void __launch_bounds__(256) distill_lanes_kernel(xrl_distill_t p) {
     float f[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) { f[j] = __builtin_amdgcn_exp2f((R::get(v[j / PER], j % PER) - m) * kt); z += f[j]; }
-    any = top(any); ts = sum(ts); z = sum(z);
+    any = lane_max<L>(any); ts = lane_sum<L>(ts); z = lane_sum<L>(z);
     const bool live = any != 0.f && m != -INFINITY && w != 0.f;
     const float lz = logf(z), lt = logf(ts), inv_t = 1.f / ts;
     float term = 0.f;
@@ -139,7 +127,7 @@ __global__ void __launch_bounds__(256) distill_lanes_kernel(xrl_distill_t p) {
             tq[k] = q;
             twice = twice || at_action[ti[k]] != k;
         }
-    term = sum(term);
+    term = lane_sum<L>(term);
     if (lane == 0) p.loss[row] = live ? w * p.temperature * p.temperature * term : 0.f;
     if (!p.d_logits) return;
     wave_lds_fence();
@@ -170,27 +158,12 @@ __global__ void __launch_bounds__(256) distill_lanes_kernel(xrl_distill_t p) {
     for (int q = 0; q < NV; ++q) distill_store<E>(d, 8 * lane + PER * q, A, f + PER * q);
 }
 
-// the sum or the maximum over a wave's lanes, by neighbours' registers (rows of 16 lanes, then across the rows), the same value for all of them
-template <bool MAX>
-__device__ __forceinline__ float wave_all(float v) {
-    const int none = __float_as_int(MAX ? -INFINITY : 0.f);
-#define WAVE_STEP(CTRL, ROWS)                                                                                                        \
-    {                                                                                                                                \
-        const float o = __int_as_float(__builtin_amdgcn_update_dpp(none, __float_as_int(v), CTRL, ROWS, 0xf, false));                \
-        v = MAX ? nan_max(v, o) : v + o;                                                                                               \
-    }
-    WAVE_STEP(0x111, 0xf) WAVE_STEP(0x112, 0xf) WAVE_STEP(0x114, 0xf) WAVE_STEP(0x118, 0xf)      // a row's lanes up to this one
-    WAVE_STEP(0x142, 0xa) WAVE_STEP(0x143, 0xc)                  // lane 15 to the next row, lane 31 to the two behind it
-#undef WAVE_STEP
-    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
-}
-
 // sums or maxima of two values over a workgroup of T threads; every call uses another part of `scratch`.  For T = 64 they are
 // over the wave, and no `scratch` is used.
 template <int T, bool MAX>
 __device__ __forceinline__ float2 block_pair(float a, float b, float2* scratch) {
-    a = wave_all<MAX>(a);
-    b = wave_all<MAX>(b);
+    a = MAX ? lane_max<64>(a) : lane_sum<64>(a);
+    b = MAX ? lane_max<64>(b) : lane_sum<64>(b);
     if (T == 64) return make_float2(a, b);
     if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = make_float2(a, b);
     lds_barrier();
@@ -278,7 +251,7 @@ __global__ void __launch_bounds__(256) distill_wave_kernel(xrl_distill_t p) {
         te[e] /= sums.y;
         if (te[e] != 0.f) term += te[e] * (((tl[e] - tm) * inv_tau - lt) - ((z_at[e] - m) * inv_tau - lz));
     }
-    term = wave_all<false>(term);
+    term = lane_sum<64>(term);
     if (lane == 0) p.loss[row] = w * p.temperature * p.temperature * term;
     if (!d) return;
     // entries that name one action: found by every entry's action in turn, which no entry without one can meet
