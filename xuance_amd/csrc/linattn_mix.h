@@ -11,8 +11,9 @@
 // LDS.  The next chunk's rows are requested into registers before the current one is multiplied.
 //
 // Precision.  f32: f32 matrix instructions throughout.  bf16: products of stored bf16 values are exact and accumulate in f32; P and S enter their
-// products as two bf16 parts (off by 2^-17 at most, the stored result by 2^-9), the weighted c enters the state as three (exact), so a state is as
-// good as f32 sums make it.  Powers of lam are made in f64; lam^64, applied to the state at every chunk, keeps its rounding error as a second float.
+// products as two bf16 parts (off by 2^-17 at most, the stored result by 2^-9), the weighted c enters the state as three (exact) where
+// the state is a result and as two where it only serves the next chunks' outputs, which are stored in bf16, so a state is as good as f32 sums make
+// it.  Powers of lam are made in f64; lam^64, applied to the state at every chunk, keeps its rounding error as a second float.
 #pragma once
 #include "io16.h"
 
@@ -44,7 +45,7 @@ template <typename E, int TS> struct mix_ops;
 // Operands by fragments: KB values of k of 16 rows or columns.  A product of fragments takes STEPS matrix instructions; an f32 operand that is made
 // here (P, the state, the weighted c) takes P_PARTS, S_PARTS, W_PARTS fragments.
 template <> struct mix_ops<float, 16> {
-    static constexpr int KB = 16, PAD = 4, SLOTS = 4, STEPS = 4, P_PARTS = 1, S_PARTS = 1, W_PARTS = 1;
+    static constexpr int KB = 16, PAD_A = 4, PAD_B = 4, PAD_C = 4, PAD_P = 4, SLOTS = 4, STEPS = 4, P_PARTS = 1, S_PARTS = 1, W_PARTS = 1;
     typedef f32x4_t frag;
     typedef f32x4_t acc;
     // four values of a row of LDS, k = 16 p + 4 g + r
@@ -68,7 +69,9 @@ template <> struct mix_ops<float, 16> {
 
 // what both tile sizes of bf16 share
 struct mix_bf16 {
-    static constexpr int PAD = 8, SLOTS = 8, STEPS = 1, P_PARTS = 2, S_PARTS = 2, W_PARTS = 3;
+    // LDS rows: read 8 bytes of each of 16 rows at a time (a), by transposing reads of 32 bytes of 4 rows (c), both (b) or 16 bytes of 8 rows (P); each wants
+    // its rows to fall behind each other in the 32 banks.  With 8 for all, half of the cycles that LDS was busy were conflicts.
+    static constexpr int PAD_A = 4, PAD_B = 8, PAD_C = 16, PAD_P = 8, SLOTS = 8, STEPS = 1, P_PARTS = 2, S_PARTS = 2, W_PARTS = 3;
     typedef u32x4_t frag;                                        // eight bf16
     static __device__ __forceinline__ u32x2_t two(const bf16_t* p) { return *reinterpret_cast<const u32x2_t*>(p); }
     static __device__ __forceinline__ frag join(u32x2_t x, u32x2_t y) { return frag{x.x, x.y, y.x, y.y}; }
@@ -240,7 +243,13 @@ struct mix_stage_t {
             E* to = lds + (reverse ? CH - 1 - row0 : row0) * STRIDE + at0;
             const int step = reverse ? -STEP * STRIDE : STEP * STRIDE;
 #pragma unroll
-            for (int q = 0; q < N; ++q) *reinterpret_cast<u32x4_t*>(to + q * step) = v[q];
+            for (int q = 0; q < N; ++q) {
+                if (STRIDE * sizeof(E) % 16 == 0) *reinterpret_cast<u32x4_t*>(to + q * step) = v[q];
+                else {
+                    *reinterpret_cast<u32x2_t*>(to + q * step) = u32x2_t{v[q].x, v[q].y};
+                    *reinterpret_cast<u32x2_t*>(to + q * step + PER / 2) = u32x2_t{v[q].z, v[q].w};
+                }
+            }
         }
     }
 };
@@ -248,8 +257,8 @@ struct mix_stage_t {
 template <typename E, int TS, int DA, int NW>
 struct mix_geom {
     typedef mix_ops<E, TS> M;
-    static constexpr int DC = TS * NW, NT = 64 * NW, SA = DA + M::PAD, SC = DC + M::PAD, SP = CH + M::PAD;
-    static constexpr int A = 0, B = A + CH * SA, C = B + CH * SA, P = C + CH * SC, END = P + M::P_PARTS * CH * SP;
+    static constexpr int DC = TS * NW, NT = 64 * NW, SA = DA + M::PAD_A, SB = DA + M::PAD_B, SC = DC + M::PAD_C, SP = CH + M::PAD_P;
+    static constexpr int A = 0, B = A + CH * SA, C = B + CH * SB, P = C + CH * SC, END = P + M::P_PARTS * CH * SP;
     static constexpr int BYTES = END * (int)sizeof(E);
     static constexpr int FIT = NW * (160 * 1024 / (BYTES + 2048)), MIN_WAVES = FIT >= 8 ? 2 : 1;      // waves of a compute unit, and so of a SIMD, that LDS has room for
 };
@@ -290,9 +299,22 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, TS, DA, NW>::MIN_WAVES))
     const int job_i = both / p.n_slices, unit = turn / (p.n_jobs * p.n_slices) * 8 + (lin & 7);
     if (unit >= p.B * p.H * p.n_seg) return;
     const mix_job_t& J = p.job[job_i];
-    const int bh = unit / p.n_seg, seg = unit % p.n_seg, b = bh / p.H, h = bh % p.H;
+    const int seg = unit % p.n_seg, h = unit / p.n_seg % p.H, nth = unit / p.n_seg / p.H;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), ln0 = lane % TS, g0 = lane / TS;
     typedef const __attribute__((address_space(4))) int* scalar_int_t;
+    int b = nth;
+    if (p.lengths && p.B <= 64) {
+        // few rows: the longest first, so that the last workgroups to end are short ones (8 ragged rows of 4096 steps, forward and backward, 432 -> 418 us;
+        // more rows even out by themselves)
+        const int mine = lane < p.B ? min(max(p.lengths[lane], 0), p.T) : -1;
+        int longer = 0;
+        for (int k = 0; k < p.B; ++k) {
+            const int other = __builtin_amdgcn_readlane(mine, k);
+            longer += other > mine || (other == mine && k < lane) ? 1 : 0;
+        }
+        b = __builtin_ctzll(__ballot(lane < p.B && longer == nth));
+    }
+    const int bh = b * p.H + h;
     const int n = p.lengths ? min(max(((scalar_int_t)(uintptr_t)p.lengths)[b], 0), p.T) : p.T;
     const int seg_chunks = ((n + CH - 1) / CH + p.n_seg - 1) / p.n_seg, c_first = seg * seg_chunks, c_end = min(c_first + seg_chunks, (n + CH - 1) / CH);
     const int c0 = (both % p.n_slices) * G::DC;                     // the slice of c's columns
@@ -304,8 +326,9 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, TS, DA, NW>::MIN_WAVES))
     E* po = (E*)J.out + b * J.so[1] + h * J.so[2] + c0;
     const int64_t so = J.so[0];
 
-    mix_stage_t<E, DA, NT, FULL, M::PAD> ra, rb;
-    mix_stage_t<E, G::DC, NT, FULL, M::PAD> rc;
+    mix_stage_t<E, DA, NT, FULL, M::PAD_A> ra;
+    mix_stage_t<E, DA, NT, FULL, M::PAD_B> rb;
+    mix_stage_t<E, G::DC, NT, FULL, M::PAD_C> rc;
     ra.begin((const E*)J.a + b * J.sa[1] + h * J.sa[2], J.sa[0], da, n, reverse);
     rb.begin((const E*)J.b + b * J.sb[1] + h * J.sb[2], J.sb[0], da, n, reverse);
     rc.begin((const E*)J.c + b * J.sc[1] + h * J.sc[2] + c0, J.sc[0], dc, n, reverse);
@@ -420,7 +443,7 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, TS, DA, NW>::MIN_WAVES))
 #pragma unroll
                     for (int r = 0; r < AR; ++r) s[k][r] = 0.f;
                     ax[k] = la + (TS * it[k] + ln) * G::SA;
-                    bx[k] = lb + (TS * jt[k] + ln) * G::SA;
+                    bx[k] = lb + (TS * jt[k] + ln) * G::SB;
                 }
                 frag fa[2][AT_ONCE], fb[2][AT_ONCE];
 #pragma unroll
@@ -533,7 +556,7 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, TS, DA, NW>::MIN_WAVES))
             frag fb[TILES];
             if (q >= 0)
 #pragma unroll
-                for (int t = 0; t < TILES; ++t) fb[t] = M::column(lb, G::SA, q, g, TS * t + ln);
+                for (int t = 0; t < TILES; ++t) fb[t] = M::column(lb, G::SB, q, g, TS * t + ln);
             float wv[M::SLOTS];
             if (q + 1 < NPC) {
 #pragma unroll
