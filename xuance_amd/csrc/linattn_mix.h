@@ -254,13 +254,21 @@ struct mix_stage_t {
     }
 };
 
+constexpr int up(int bytes) { return (bytes + 1279) / 1280 * 1280; }                   // LDS is given out in pieces of this size
+
 template <typename E, int TS, int DA, int NW>
 struct mix_geom {
     typedef mix_ops<E, TS> M;
     static constexpr int DC = TS * NW, NT = 64 * NW, SA = DA + M::PAD_A, SB = DA + M::PAD_B, SC = DC + M::PAD_C, SP = CH + M::PAD_P;
-    static constexpr int A = 0, B = A + CH * SA, C = B + CH * SB, P = C + CH * SC, END = P + M::P_PARTS * CH * SP;
-    static constexpr int BYTES = END * (int)sizeof(E);
-    static constexpr int FIT = NW * (160 * 1024 / (BYTES + 2048)), MIN_WAVES = FIT >= 8 ? 2 : 1;      // waves of a compute unit, and so of a SIMD, that LDS has room for
+    static constexpr int P_SIZE = M::P_PARTS * CH * SP, P_TILES = (CH / TS) * (CH / TS + 1) / 2, MINE = (P_TILES + NW - 1) / NW;
+    // P in the place of A, which costs a barrier, where a wave's tiles of P fit its registers and a third workgroup fits the compute unit for it:
+    // 256 rows of 256 steps, 4 heads of 64, f32, forward and backward 387 us with two workgroups, 370 with three
+    static constexpr int OTHER = 1280, OVER_SIZE = P_SIZE > CH * SA ? P_SIZE : CH * SA;
+    static constexpr bool OVER = M::KB == TS && MINE <= 3 && 160 * 1024 / up((CH * (SA + SB + SC) + P_SIZE) * (int)sizeof(E) + OTHER) == 2 &&
+                                 160 * 1024 / up((OVER_SIZE + CH * (SB + SC)) * (int)sizeof(E) + OTHER) == 3;
+    static constexpr int A = 0, B = A + (OVER ? OVER_SIZE : CH * SA), C = B + CH * SB, P = OVER ? A : C + CH * SC, END = OVER ? C + CH * SC : P + P_SIZE;
+    static constexpr int BYTES = END * (int)sizeof(E), HELD = 160 * 1024 / up(BYTES + OTHER);          // workgroups that LDS has room for
+    static constexpr int MIN_WAVES = OVER ? 3 : NW * HELD >= 8 ? 2 : 1;
 };
 
 // between scheduling fences: V vector instructions behind each of N matrix instructions, which run meanwhile
@@ -290,10 +298,11 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, TS, DA, NW>::MIN_WAVES))
     E* lb = reinterpret_cast<E*>(lds_raw) + G::B;
     E* lc = reinterpret_cast<E*>(lds_raw) + G::C;
     E* lp = reinterpret_cast<E*>(lds_raw) + G::P;
-    // powers of lam: 0..64 and that of the last chunk's steps; those of the scores by i - j + 32, 0 for i < j; weights of a S and of c by step, of
+    // powers of lam: 0..64 and that of the last chunk's steps (of the last two also the rounding error); those of the scores by i - j + 32, 0 for i < j; weights of c by step, of
     // whole chunks without a cut [0] and of the chunk at hand otherwise [1]
-    __shared__ float pw[CH + 2], pw_low[CH + 2], score_w[CH + 32], wq[2][CH], wb[2][CH];
-    __shared__ int seg_of[CH];
+    __shared__ float pw[CH + 2], pw_low[2], score_w[CH + 32], wb[2][CH];
+    __shared__ unsigned char seg_of[CH];
+    static_assert(sizeof(pw) + sizeof(pw_low) + sizeof(score_w) + sizeof(wb) + sizeof(seg_of) <= G::OTHER, "LDS");
     // workgroups of one row and head follow each other on one XCD (ids go round the 8 of them): its jobs share their reads in that L2
     const int lin = blockIdx.x, turn = lin >> 3, both = turn % (p.n_jobs * p.n_slices);
     const int job_i = both / p.n_slices, unit = turn / (p.n_jobs * p.n_slices) * 8 + (lin & 7);
@@ -352,7 +361,7 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, TS, DA, NW>::MIN_WAVES))
     for (int k = tid; k < CH + 2; k += NT) {
         const double f = exp((double)gl * (k <= CH ? k : n_last));
         pw[k] = (float)f;
-        pw_low[k] = (float)(f - (double)(float)f);
+        if (k >= CH) pw_low[k - CH] = (float)(f - (double)(float)f);
     }
     acc S[TILES];
     {
@@ -397,7 +406,6 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, TS, DA, NW>::MIN_WAVES))
     lds_barrier();
     for (int k = tid; k < CH + 32; k += NT) score_w[k] = k < 32 ? 0.f : scale_p * pw[k - 32];
     if (tid < CH) {
-        wq[0][tid] = scale_s * pw[tid + off];
         wb[0][tid] = scale_b * pw[CH - tid - off];
     }
 
@@ -418,9 +426,8 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, TS, DA, NW>::MIN_WAVES))
         const int own_w = cuts != 0 || left < CH ? 1 : 0;
         if (own_w && tid < CH) {
             const int nv = min(left, CH), k = __popcll(cuts & (~0ull >> (63 - tid)));      // cuts up to and including this step
-            const float q = pw[tid + off], x = pw[max(nv - tid - off, 0)];
-            seg_of[tid] = k;
-            wq[1][tid] = k == 0 ? scale_s * q : 0.f;
+            const float x = pw[max(nv - tid - off, 0)];
+            seg_of[tid] = (unsigned char)k;
             wb[1][tid] = tid < nv && k == __popcll(cuts) ? scale_b * x : 0.f;
         }
         lds_barrier();
@@ -428,11 +435,20 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, TS, DA, NW>::MIN_WAVES))
         acc O[IT];
         if (!states_only) {
             // P^T tiles on and below the diagonal, dealt out to the waves, up to three at a time
-            constexpr int ALL_P = IT * (IT + 1) / 2, MINE = (ALL_P + NW - 1) / NW, AT_ONCE = MINE < 3 ? MINE : 3;
+            constexpr int ALL_P = G::P_TILES, MINE = G::MINE, AT_ONCE = MINE < 3 ? MINE : 3;
+            acc s[AT_ONCE];
+            int it[AT_ONCE], jt[AT_ONCE];
+            auto store_scores = [&](int t0) {
+#pragma unroll
+                for (int k = 0; k < AT_ONCE; ++k)
+#pragma unroll
+                    for (int x = 0; x < QUADS; ++x)
+                        if (t0 + k < MINE)
+                            M::store_p(lp + (TS * it[k] + ln) * G::SP + TS * jt[k] + 8 * x + 4 * g, PLANE,
+                                       f32x4_t{s[k][4 * x], s[k][4 * x + 1], s[k][4 * x + 2], s[k][4 * x + 3]});
+            };
 #pragma unroll
             for (int t0 = 0; t0 < MINE; t0 += AT_ONCE) {
-                acc s[AT_ONCE];
-                int it[AT_ONCE], jt[AT_ONCE];
                 const E *ax[AT_ONCE], *bx[AT_ONCE];
                 float sw[AT_ONCE][AR];
 #pragma unroll
@@ -478,13 +494,7 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, TS, DA, NW>::MIN_WAVES))
                         for (int r = 0; r < AR; ++r) s[k][r] = seg_of[TS * jt[k] + 8 * (r >> 2) + 4 * g + (r & 3)] == m ? s[k][r] : 0.f;
                     }
                 }
-#pragma unroll
-                for (int k = 0; k < AT_ONCE; ++k)
-#pragma unroll
-                    for (int x = 0; x < QUADS; ++x)
-                        if (t0 + k < MINE)
-                            M::store_p(lp + (TS * it[k] + ln) * G::SP + TS * jt[k] + 8 * x + 4 * g, PLANE,
-                                       f32x4_t{s[k][4 * x], s[k][4 * x + 1], s[k][4 * x + 2], s[k][4 * x + 3]});
+                if (!G::OVER) store_scores(t0);
             }
 #pragma unroll
             for (int it = 0; it < IT; ++it)
@@ -497,7 +507,7 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, TS, DA, NW>::MIN_WAVES))
 #pragma unroll
                 for (int it = 0; it < IT; ++it) {
                     if (q + 1 < NPA) fa[(q + 1) & 1][it] = M::row(la + (TS * it + ln) * G::SA, q + 1, g);
-                    else fq[it] = wq[own_w][TS * it + ln];
+                    else fq[it] = scale_s * (cuts && seg_of[TS * it + ln] != 0 ? 0.f : pw[TS * it + ln + off]);
                 }
                 if (q >= 0) {
 #pragma unroll
@@ -514,10 +524,14 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, TS, DA, NW>::MIN_WAVES))
             for (int it = 0; it < IT; ++it)
 #pragma unroll
                 for (int r = 0; r < AR; ++r) O[it][r] *= fq[it];
+            if (G::OVER) {
+                lds_barrier();                                       // A has been read by all
+                store_scores(0);
+            }
             lds_barrier();
         }
         const bool last = left <= CH;
-        const float ch = cuts ? 0.f : pw[last ? CH + 1 : CH], cl = cuts ? 0.f : pw_low[last ? CH + 1 : CH];
+        const float ch = cuts ? 0.f : pw[last ? CH + 1 : CH], cl = cuts ? 0.f : pw_low[last ? 1 : 0];
         // where half of the state or more is gone a chunk later, the rounding of lam^64 does not add up over the chunks
         const bool two = __builtin_amdgcn_readfirstlane(ch > 0.5f);
         frag cf[NPC];
@@ -652,7 +666,7 @@ static int launch_mix_size(const mix_t& m, int dc, hipStream_t s) {
 template <typename E, int TS, int DA, int NW>
 static int mix_resident() {
     typedef mix_geom<E, TS, DA, NW> G;
-    const int by_lds = 160 * 1024 / (G::BYTES + 2560), by_registers = 8 / NW > 0 ? 8 / NW : 1;
+    const int by_lds = G::HELD, by_registers = (G::OVER ? 12 : 8) / NW > 0 ? (G::OVER ? 12 : 8) / NW : 1;
     return by_lds < by_registers ? by_lds : by_registers;
 }
 
