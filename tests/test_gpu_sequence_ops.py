@@ -176,6 +176,37 @@ def test_linattn_long_axis_split_over_workgroups(ops, T, B, H, dk, dv, dtype):
     lin_check(c, lin_run(ops, c))
 
 
+@pytest.mark.parametrize("lengths", [[600, 600, 600, 600], [0, 0, 0, 0], [1, 900, 64, 640], [-5, 0, 580, 4000], "65 rows"])
+def test_linattn_rows_of_many_orders(ops, lengths):
+    """Rows are taken up by their lengths: equal ones, none, ascending, out of range (cut to 0 and T), more rows than a wave has lanes."""
+    B = 65 if lengths == "65 rows" else len(lengths)
+    T = 70 if B == 65 else 640
+    c = lin_case(B, T, B, 2, 16, 16, F32, "ragged", B < 65, True)
+    c["lengths"] = torch.randint(0, T + 1, (B,), generator=gen(3), dtype=torch.int32) if B == 65 else torch.tensor(lengths, dtype=torch.int32)
+    got = lin_run(ops, c)
+    c["lengths"] = c["lengths"].clamp(0, T)
+    lin_check(c, got)
+
+
+def test_linattn_two_calls_at_once(ops):
+    """Two streams, each with a workspace of its own."""
+    cases = [lin_case(50 + i, 1300, 1, 2, 64, 64, F32, None, True, True) for i in range(2)]
+    plain = [lin_run(ops, c) for c in cases]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    dev = [{n: (t.cuda() if isinstance(t, torch.Tensor) else t) for n, t in c.items()} for c in cases]
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(4):
+        for d, s in zip(dev, streams):
+            with torch.cuda.stream(s):
+                out = torch.empty_like(d["v"])
+                ops.linattn_forward(d["q"], d["k"], d["v"], out, d["log_decay"], scale=d["scale"], reset=d["reset"], state=d["state"])
+                outs.append(out)
+    torch.cuda.synchronize()
+    for i, out in enumerate(outs):
+        assert torch.equal(out, plain[i % 2]["out"])
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
 def test_linattn_decays_at_both_ends(ops, dtype):
     """No decay, no memory at all, and decays whose powers leave the range of f32 within one chunk; a positive one is taken as 0."""
@@ -530,6 +561,12 @@ def test_block_norm_many_rows(ops):
     norm_check(ops, norm_case(7, 5003, 520, BF16), "layer")
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("N,D", [(1700, 2048), (1801, 1999), (600, 8192), (2100, 512)])
+def test_block_norm_more_wide_rows_than_workgroups(ops, N, D, dtype):
+    norm_check(ops, norm_case(N, N, D, dtype), "layer")
+
+
 def odd_rows(t):
     wide = torch.full((t.shape[0], t.shape[1] + 5), 3.0, device=t.device, dtype=t.dtype)
     wide[:, 1:-4] = t
@@ -765,6 +802,35 @@ def test_distill_nan_reaches_the_result(ops, A, dtype):
             assert torch.isnan(d[row].float()).all() if row != 4 else torch.isnan(d[row, c["teacher_idx"][4].long().cuda()].float()).all()
         else:
             assert torch.equal(loss[row], want[0][row]) and torch.equal(d[row], want[1][row])
+
+
+@pytest.mark.parametrize("N,A,dtype", [(1200, 20000, F32), (1100, 13000, BF16), (700, 33000, BF16)])
+def test_distill_more_wide_rows_than_workgroups(ops, N, A, dtype):
+    """A workgroup takes several rows and requests the next one ahead: rows of weight 0, without entries and without actions in between."""
+    c = distill_case(15, N, A, 9, dtype, avail=True)
+    c["weight"][::3] = 0.0
+    c["logits"][::3] = math.nan
+    c["teacher_idx"][1::7] = -1
+    c["avail"][2::11] = 0.0
+    loss, d = distill_check(ops, c)
+    assert (loss[::3] == 0).all() and (d[::3] == 0).all()
+
+
+def test_distill_wide_rows_captured(ops):
+    from xuance_amd.ops import Graph
+    c = distill_case(16, 40, 25000, 12)
+    dev = {n: t.cuda() for n, t in c.items() if t is not None}
+    loss, d = torch.zeros(40, device="cuda"), torch.zeros(40, 25000, device="cuda")
+    graph = Graph()
+    with graph:
+        ops.distill_loss(dev["logits"], dev["teacher_idx"], dev["teacher_logits"], loss, d_logits=d, weight=dev["weight"], temperature=2.0, grad_scale=0.5)
+    want = distill_run(ops, c, 2.0, 0.5)
+    for _ in range(3):
+        loss.fill_(7.0)
+        d.fill_(7.0)
+        graph.launch()
+        torch.cuda.synchronize()
+        assert torch.equal(loss, want[0]) and torch.equal(d, want[1])
 
 
 def test_distill_layout_in_place_and_loss_only(ops):
