@@ -29,6 +29,7 @@ struct mix_job_t {
     int reverse, off;
     float scale_p, scale_s, scale_b;      // of the products a.b, of a S, of b (x) c in the state
     float* carry;                         // pass over the states of segments: what a segment multiplies the state by
+    int fine;                             // ...: a state that the call gives back comes of it
 };
 struct mix_t {
     mix_job_t job[3];
@@ -383,7 +384,7 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, TS, DA, NW>::MIN_WAVES))
                 }
         }
     }
-    const bool fine = states_only || (J.s_out && p.n_seg == 1);      // the state is a result
+    const bool fine = states_only ? J.fine != 0 : J.s_out && p.n_seg == 1;      // the state is a result
     if (!states_only) {
         // P's tiles above the diagonal that share a fragment with one on it are read and stay 0
         if (M::KB > TS)
