@@ -1,0 +1,78 @@
+"""Numerics of the sequence-policy operators that a bound on random values does not see: cases whose sums are exact in f32."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from xuance_amd import ops
+    torch.cuda.set_device(0)
+    ops.init_device()
+    return ops
+
+
+def gen(seed):
+    g = torch.Generator()
+    g.manual_seed(seed)
+    return g
+
+
+# ------------------------------------------------------------------------------------------------------- linear attention
+def lin(ops, q, k, v, d_out, log_decay, state=None, d_state_out=None, reset=None, lengths=None, scale=1.0, results=True):
+    """Both passes on the device; results: ask for the states too."""
+    c = lambda t: None if t is None else t.cuda()                                    # noqa: E731
+    q, k, v, d_out, ld = c(q), c(k), c(v), c(d_out), c(torch.as_tensor(log_decay, dtype=F32))
+    T, B, H, dk = q.shape
+    s = lambda: torch.full((B, H, dk, v.shape[3]), 7.5, device="cuda")              # noqa: E731
+    par = dict(scale=scale, lengths=c(lengths), reset=c(reset), state=c(state))
+    r = dict(out=torch.empty_like(v))
+    if results:
+        r["state_out"] = s()
+    ops.linattn_forward(q, k, v, r["out"], ld, state_out=r.get("state_out"), **par)
+    r.update(d_q=torch.empty_like(q), d_k=torch.empty_like(k), d_v=torch.empty_like(v))
+    if results:
+        r["d_state"] = s()
+    ops.linattn_backward(q, k, v, d_out, r["d_q"], r["d_k"], r["d_v"], ld, d_state_out=c(d_state_out), d_state=r.get("d_state"), **par)
+    torch.cuda.synchronize()
+    return {n: t.cpu() for n, t in r.items()}
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("d", [4, 32, 64, 128])
+def test_linattn_products_keep_the_bits_of_f32(ops, d, dtype):
+    """Scores and states of 21 bits against ones that take all but the last of them away again: every sum is exact in f32, in any order."""
+    a, rest = 1 + 2.0 ** -10 + 2.0 ** -20, 2.0 ** -20
+    z = lambda T: torch.zeros(T, 1, 1, d, dtype=dtype)                               # noqa: E731
+    # scores: q_1 k_0 = a, q_1 k_1 = a - rest, v_0 = 1, v_1 = -1; the same numbers through v and d_out give d_q
+    q, k, v, do = z(2), z(2), z(2), z(2)
+    row = torch.tensor([1, 2.0 ** -10, 2.0 ** -20], dtype=dtype)
+    q[1, 0, 0, :3], k[0, 0, 0, :3], k[1, 0, 0, :2] = row, 1, 1
+    v[0], v[1] = 1, -1
+    assert (lin(ops, q, k, v, do, [0.0])["out"][1] == rest).all()
+    q, k, v, do = z(2), z(2), z(2), z(2)
+    do[1, 0, 0, :3], v[0, 0, 0, :3], v[1, 0, 0, :2] = row, 1, 1
+    k[0], k[1] = 1, -1
+    assert (lin(ops, q, k, v, do, [0.0])["d_q"][1] == rest).all()
+    # states: rows a and -(a - rest), both read with weight 1
+    S = torch.zeros(1, 1, d, d)
+    S[0, 0, 0], S[0, 0, 1] = a, rest - a
+    x = z(1)
+    x[0, 0, 0, :2] = 1
+    assert (lin(ops, x, z(1), z(1), z(1), [0.0], state=S)["out"] == rest).all()
+    assert (lin(ops, z(1), x, z(1), z(1), [0.0], d_state_out=S)["d_v"] == rest).all()
+    assert (lin(ops, z(1), z(1), z(1), x, [0.0], state=S.transpose(2, 3).contiguous())["d_q"] == rest).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("d", [16, 64, 128])
+@pytest.mark.parametrize("T,B", [(300, 3), (1300, 1)])
+def test_linattn_outputs_do_not_depend_on_the_states_asked_for(ops, T, B, d, dtype):
+    g = gen(T + d)
+    q, k, v, do = (torch.randn(T, B, 2, d, generator=g).to(dtype) for _ in range(4))
+    a, b = (lin(ops, q, k, v, do, [-0.01, -0.2], scale=d ** -0.5, results=r) for r in (True, False))
+    for n in b:
+        assert torch.equal(a[n], b[n]), n

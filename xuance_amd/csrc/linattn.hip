@@ -212,7 +212,6 @@ static int run_jobs(const xrl_linattn_t& p, mix_t& m, int n_jobs, const int* hol
         mix_job_t& t = st.job[slot[i]];
         t = j;
         t.s_in = nullptr;
-        t.fine = j.s_out != nullptr;
         t.s_out = p.workspace + slot[i] * bhs * m.kv;
         t.carry = carries + slot[i] * bhs * 2;
         scan_job_t& q = sc.job[slot[i]];

@@ -10,10 +10,10 @@
 // S^T of the first product, and P^T as returned leaves for LDS with four neighbouring j per lane.  So only the chunk's a, b, c and P pass through
 // LDS.  The next chunk's rows are requested into registers before the current one is multiplied.
 //
-// Precision.  f32: f32 matrix instructions throughout.  bf16: products of stored bf16 values are exact and accumulate in f32; P and S enter their
-// products as two bf16 parts (off by 2^-17 at most, the stored result by 2^-9), the weighted c enters the state as three (exact) where
-// the state is a result and as two where it only serves the next chunks' outputs, which are stored in bf16, so a state is as good as f32 sums make
-// it.  Powers of lam are made in f64; lam^64, applied to the state at every chunk, keeps its rounding error as a second float.
+// Precision.  f32: f32 matrix instructions throughout.  bf16: products of stored bf16 values are exact and accumulate in f32; the f32 operands that
+// are made here (P, S, the weighted c) enter their products as three bf16 parts, which together are the f32 value (csrc/split3.h).  So either type
+// computes what f32 sums make of its inputs, and a bf16 result is rounded once, where it is stored.  Powers of lam are made in f64; lam^64, applied
+// to the state at every chunk, keeps its rounding error as a second float.
 //
 // Bound.  f32: the matrix instructions (half of a large product's rate): 256 rows x 256 steps, 4 heads of 64: 98 us forward, 280 us the three gradients.
 // bf16, heads of 128: a chunk takes a compute unit 9.7 k cycles, 27% of them matrix instructions, 36% vector instructions (two-part operands, decays),
@@ -34,7 +34,6 @@ struct mix_job_t {
     int reverse, off;
     float scale_p, scale_s, scale_b;      // of the products a.b, of a S, of b (x) c in the state
     float* carry;                         // pass over the states of segments: what a segment multiplies the state by
-    int fine;                             // ...: a state that the call gives back comes of it
 };
 struct mix_t {
     mix_job_t job[3];
@@ -65,7 +64,7 @@ template <> struct mix_ops<float, 16> {
     }
     static __device__ __forceinline__ acc mfma(frag a, frag b, acc c, int step) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a[step], b[step], c, 0, 0, 0); }
     static __device__ __forceinline__ void of_state(const acc* s, int p, frag (&f)[1]) { f[0] = s[p]; }
-    static __device__ __forceinline__ void weigh(frag v, const float* w, frag (&f)[1], bool) {
+    static __device__ __forceinline__ void weigh(frag v, const float* w, frag (&f)[1]) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) f[0][r] = v[r] * w[r];
     }
@@ -77,7 +76,7 @@ template <> struct mix_ops<float, 16> {
 struct mix_bf16 {
     // LDS rows: read 8 bytes of each of 16 rows at a time (a), by transposing reads of 32 bytes of 4 rows (c), both (b) or 16 bytes of 8 rows (P); each wants
     // its rows to fall behind each other in the 32 banks.  With 8 for all, half of the cycles that LDS was busy were conflicts.
-    static constexpr int PAD_A = 4, PAD_B = 8, PAD_C = 16, PAD_P = 8, SLOTS = 8, STEPS = 1, P_PARTS = 2, S_PARTS = 2, W_PARTS = 3;
+    static constexpr int PAD_A = 4, PAD_B = 8, PAD_C = 16, PAD_P = 8, SLOTS = 8, STEPS = 1, P_PARTS = 3, S_PARTS = 3, W_PARTS = 3;
     typedef u32x4_t frag;                                        // eight bf16
     static __device__ __forceinline__ u32x2_t two(const bf16_t* p) { return *reinterpret_cast<const u32x2_t*>(p); }
     static __device__ __forceinline__ frag join(u32x2_t x, u32x2_t y) { return frag{x.x, x.y, y.x, y.y}; }
@@ -90,30 +89,22 @@ struct mix_bf16 {
         return join(__builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)at)),
                     __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)(at + 4 * stride))));
     }
-    static __device__ __forceinline__ void split2(float x0, float x1, unsigned& h, unsigned& l) {
-        h = cvt_pk_bf16(x0, x1);
-        l = cvt_pk_bf16(x0 - __uint_as_float(h << 16), x1 - __uint_as_float(h & 0xffff0000u));
-    }
-    // the third part where the state is a result
-    static __device__ __forceinline__ void weigh(frag v, const float* w, frag (&f)[3], bool third) {
+    static __device__ __forceinline__ void weigh(frag v, const float* w, frag (&f)[3]) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            const float x = __uint_as_float(v[q] << 16) * w[2 * q], y = __uint_as_float(v[q] & 0xffff0000u) * w[2 * q + 1];
-            unsigned hi, lo;
-            split2(x, y, hi, lo);
-            f[0][q] = hi; f[1][q] = lo;
-            if (third)
-                f[2][q] = cvt_pk_bf16((x - __uint_as_float(hi << 16)) - __uint_as_float(lo << 16),
-                                      (y - __uint_as_float(hi & 0xffff0000u)) - __uint_as_float(lo & 0xffff0000u));
+            unsigned h, m, l;
+            split3_pair(__uint_as_float(v[q] << 16) * w[2 * q], __uint_as_float(v[q] & 0xffff0000u) * w[2 * q + 1], h, m, l);
+            f[0][q] = h; f[1][q] = m; f[2][q] = l;
         }
     }
     static __device__ __forceinline__ void store_p(bf16_t* p, int plane, f32x4_t v) {
-        unsigned h0, l0, h1, l1;
-        split2(v[0], v[1], h0, l0);
-        split2(v[2], v[3], h1, l1);
-        const u32x2_t h = {h0, h1}, l = {l0, l1};
+        unsigned h0, m0, l0, h1, m1, l1;
+        split3_pair(v[0], v[1], h0, m0, l0);
+        split3_pair(v[2], v[3], h1, m1, l1);
+        const u32x2_t h = {h0, h1}, m = {m0, m1}, l = {l0, l1};
         *reinterpret_cast<u32x2_t*>(p) = h;
-        *reinterpret_cast<u32x2_t*>(p + plane) = l;
+        *reinterpret_cast<u32x2_t*>(p + plane) = m;
+        *reinterpret_cast<u32x2_t*>(p + 2 * plane) = l;
     }
     static __device__ __forceinline__ void store_out(bf16_t* o, f32x4_t v) {
         typedef u32x2_t any_t __attribute__((aligned(2)));
@@ -133,13 +124,13 @@ template <> struct mix_ops<bf16_t, 16> : mix_bf16 {
     static __device__ __forceinline__ acc mfma(frag a, frag b, acc c, int) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
     }
-    static __device__ __forceinline__ void of_state(const acc* s, int p, frag (&f)[2]) {
+    static __device__ __forceinline__ void of_state(const acc* s, int p, frag (&f)[3]) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const acc t = s[2 * p + (q >> 1)];
-            unsigned x, y;
-            split2(t[2 * (q & 1)], t[2 * (q & 1) + 1], x, y);
-            f[0][q] = x; f[1][q] = y;
+            unsigned h, m, l;
+            split3_pair(t[2 * (q & 1)], t[2 * (q & 1) + 1], h, m, l);
+            f[0][q] = h; f[1][q] = m; f[2][q] = l;
         }
     }
 };
@@ -157,12 +148,12 @@ template <> struct mix_ops<bf16_t, 32> : mix_bf16 {
     static __device__ __forceinline__ acc mfma(frag a, frag b, acc c, int) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
     }
-    static __device__ __forceinline__ void of_state(const acc* s, int p, frag (&f)[2]) {
+    static __device__ __forceinline__ void of_state(const acc* s, int p, frag (&f)[3]) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            unsigned x, y;
-            split2(s[p >> 1][8 * (p & 1) + 2 * q], s[p >> 1][8 * (p & 1) + 2 * q + 1], x, y);
-            f[0][q] = x; f[1][q] = y;
+            unsigned h, m, l;
+            split3_pair(s[p >> 1][8 * (p & 1) + 2 * q], s[p >> 1][8 * (p & 1) + 2 * q + 1], h, m, l);
+            f[0][q] = h; f[1][q] = m; f[2][q] = l;
         }
     }
 };
@@ -389,7 +380,6 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, TS, DA, NW>::MIN_WAVES))
                 }
         }
     }
-    const bool fine = states_only ? J.fine != 0 : J.s_out && p.n_seg == 1;      // the state is a result
     if (!states_only) {
         // P's tiles above the diagonal that share a fragment with one on it are read and stay 0
         if (M::KB > TS)
@@ -524,7 +514,7 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, TS, DA, NW>::MIN_WAVES))
                             for (int it = 0; it < IT; ++it) O[it] = M::mfma(fs[q & 1][part], fa[q & 1][it], O[it], x);
                 }
                 if (q + 1 < NPA) M::of_state(S, q + 1, fs[(q + 1) & 1]);
-                if (TS == 32) mix_interleave<IT * M::S_PARTS, 6>(q >= 0 && q + 1 < NPA);
+                if (TS == 32) mix_interleave<IT * M::S_PARTS, 8>(q >= 0 && q + 1 < NPA);
             }
 #pragma unroll
             for (int it = 0; it < IT; ++it)
@@ -585,15 +575,14 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, TS, DA, NW>::MIN_WAVES))
             if (q >= 0) {
 #pragma unroll
                 for (int part = M::W_PARTS - 1; part >= 0; --part) {
-                    if (part == 2 && !fine) continue;
 #pragma unroll
                     for (int x = 0; x < M::STEPS; ++x)
 #pragma unroll
                         for (int t = 0; t < TILES; ++t) S[t] = M::mfma(fb[t], cw[q & 1][part], S[t], x);
                 }
             }
-            if (q + 1 < NPC) M::weigh(cf[q + 1], wv, cw[(q + 1) & 1], fine);
-            if (TS == 32) mix_interleave<TILES * 2, 7>(q >= 0 && q + 1 < NPC);
+            if (q + 1 < NPC) M::weigh(cf[q + 1], wv, cw[(q + 1) & 1]);
+            if (TS == 32) mix_interleave<TILES * M::W_PARTS, 5>(q >= 0 && q + 1 < NPC);
         }
         if (!states_only) {
             // rows of O in the order of memory, as the stage's
