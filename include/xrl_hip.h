@@ -1526,7 +1526,9 @@ enum { XRL_F32 = 0, XRL_BF16 = 1 };
  * Activations are [T][B][H][d] with any strides over T, B and H (elements, 64 bits; d contiguous): stride_*[0] = from step to step,
  * [1] = from row to row, [2] = from head to head.  Stride 0 shares an input among heads or rows; outputs need every element of their own
  * and overlap no input.  lengths: steps at and behind lengths[b] are not read, take no part and their outputs are written as 0;
- * state_out is S after step lengths[b] - 1.  Inputs have to be finite: a NaN or infinity reaches the 64 steps around its own. */
+ * state_out is S after step lengths[b] - 1.  A reset ends whatever the state has become, infinities and NaN too (an overflow, a state that was
+ * given).  q, k, v and d_out have to be finite within their lengths: a NaN or infinity there reaches the other steps of its 64 (counted from the
+ * row's first step; from its last for the gradients of k and v) and, through the state, all that follow these, resets or not. */
 typedef struct {
     const void* q;           /* [T][B][H][dk] */
     const void* k;           /* [T][B][H][dk] */

@@ -76,3 +76,54 @@ def test_linattn_outputs_do_not_depend_on_the_states_asked_for(ops, T, B, d, dty
     a, b = (lin(ops, q, k, v, do, [-0.01, -0.2], scale=d ** -0.5, results=r) for r in (True, False))
     for n in b:
         assert torch.equal(a[n], b[n]), n
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("d", [16, 64, 128])
+@pytest.mark.parametrize("T,B", [(150, 3), (1300, 2)])
+def test_linattn_reset_ends_any_state(ops, T, B, d, dtype):
+    """A NaN or infinite state, given or overflowed, ends at a reset like any other: the rest of the row has the bits that it has without it."""
+    g = gen(T + d)
+    q, k, v, do = (torch.randn(T, B, 2, d, generator=g).to(dtype) for _ in range(4))
+    S, dS = torch.randn(B, 2, d, d, generator=g), torch.randn(B, 2, d, d, generator=g)
+    reset = torch.zeros(T, B)
+    reset[0, 0] = reset[T // 2, 1] = reset[T // 2 + 3, 0] = 1
+    par = dict(log_decay=[-0.01, -0.2], reset=reset, scale=d ** -0.5)
+    S[0] = 0.0
+    want = lin(ops, q, k, v, do, state=S, d_state_out=dS, **par)
+    for bad in (torch.nan, torch.inf):
+        S0 = S.clone()
+        S0[0] = bad                                                                  # reset before the first step
+        got = lin(ops, q, k, v, do, state=S0, d_state_out=dS, **par)
+        for n in want:
+            assert torch.equal(got[n], want[n]), (n, bad)
+        S1, dS1 = S.clone(), dS.clone()
+        S1[1], dS1[0] = bad, bad                                                     # ends in the middle: after it; before it for its gradient
+        got = lin(ops, q, k, v, do, state=S1, d_state_out=dS1, **par)
+        half = T // 2
+        for n in ("out", "d_q"):
+            assert torch.equal(got[n][half:], want[n][half:]) and torch.equal(got[n][:, 0], want[n][:, 0]), (n, bad)
+            assert not torch.isfinite(got[n][:half, 1].float()).all()
+        for n in ("d_k", "d_v"):
+            assert torch.equal(got[n][:half + 3], want[n][:half + 3]) and torch.equal(got[n][:, 1], want[n][:, 1]), (n, bad)
+            assert not torch.isfinite(got[n][half + 3:, 0].float()).all()
+        assert torch.equal(got["state_out"], want["state_out"]) and torch.equal(got["d_state"], want["d_state"]), bad
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("d", [16, 64, 128])
+@pytest.mark.parametrize("at", [3, 60, 64, 100])
+@pytest.mark.parametrize("T", [200, 1300])
+def test_linattn_overflow_of_one_episode_stays_in_it(ops, T, at, d, dtype):
+    """Finite keys and values whose product is not: the steps behind the next reset have the bits that they have without them."""
+    g = gen(T + d + at)
+    q, k, v, do = (torch.randn(T, 1, 1, d, generator=g).to(dtype) for _ in range(4))
+    reset = torch.zeros(T, 1)
+    reset[at + 5] = 1
+    want = lin(ops, q, k, v, do, [-0.01], reset=reset)
+    k[at], v[at] = 1e30, 1e30
+    got = lin(ops, q, k, v, do, [-0.01], reset=reset)
+    for n in ("out", "d_q", "d_k", "d_v"):
+        assert torch.equal(got[n][at + 5:], want[n][at + 5:]), n
+    assert torch.equal(got["state_out"], want["state_out"])
+    assert not torch.isfinite(got["out"][at:at + 5].float()).all()

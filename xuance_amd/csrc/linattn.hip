@@ -40,7 +40,8 @@ __global__ void __launch_bounds__(256) linattn_scan_kernel(scan_t p) {
         for (int q = 0; q < 8; ++q)
             if (i + q < p.n_seg) {
                 s[(int64_t)(i + q) * p.kv] = cur;
-                cur = __builtin_fmaf(cur, c[2 * (i + q)], cur * c[2 * (i + q) + 1]) + own[q];
+                const float keep = c[2 * (i + q)];
+                cur = keep < 0.f ? own[q] : __builtin_fmaf(cur, keep, cur * c[2 * (i + q) + 1]) + own[q];
             }
     }
     if (J.s_out) {

@@ -33,7 +33,7 @@ struct mix_job_t {
     int64_t s_row;                        // s_in: from row and head (and segment) to the next
     int reverse, off;
     float scale_p, scale_s, scale_b;      // of the products a.b, of a S, of b (x) c in the state
-    float* carry;                         // pass over the states of segments: what a segment multiplies the state by
+    float* carry;                         // pass over the states of segments: what a segment multiplies the state by; below 0 where a reset ends it
 };
 struct mix_t {
     mix_job_t job[3];
@@ -503,7 +503,7 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, TS, DA, NW>::MIN_WAVES))
 #pragma unroll
                 for (int it = 0; it < IT; ++it) {
                     if (q + 1 < NPA) fa[(q + 1) & 1][it] = M::row(la + (TS * it + ln) * G::SA, q + 1, g);
-                    else fq[it] = scale_s * (cuts && seg_of[TS * it + ln] != 0 ? 0.f : pw[TS * it + ln + off]);
+                    else fq[it] = scale_s * pw[TS * it + ln + off];
                 }
                 if (q >= 0) {
 #pragma unroll
@@ -520,6 +520,13 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, TS, DA, NW>::MIN_WAVES))
             for (int it = 0; it < IT; ++it)
 #pragma unroll
                 for (int r = 0; r < AR; ++r) O[it][r] *= fq[it];
+            if (cuts)                                                // a choice, no factor of 0: the state that a reset ends may be anything
+#pragma unroll
+                for (int it = 0; it < IT; ++it) {
+                    const bool after = seg_of[TS * it + ln] != 0;
+#pragma unroll
+                    for (int r = 0; r < AR; ++r) O[it][r] = after ? 0.f : O[it][r];
+                }
             if (G::OVER) {
                 lds_barrier();                                       // A has been read by all
                 store_scores(0);
@@ -527,7 +534,7 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, TS, DA, NW>::MIN_WAVES))
             lds_barrier();
         }
         const bool last = left <= CH;
-        const float ch = cuts ? 0.f : pw[last ? CH + 1 : CH], cl = cuts ? 0.f : pw_low[last ? 1 : 0];
+        const float ch = pw[last ? CH + 1 : CH], cl = pw_low[last ? 1 : 0];
         // where half of the state or more is gone a chunk later, the rounding of lam^64 does not add up over the chunks
         const bool two = __builtin_amdgcn_readfirstlane(ch > 0.5f);
         frag cf[NPC];
@@ -551,7 +558,10 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, TS, DA, NW>::MIN_WAVES))
                             if (q * M::KB < TS * (it + 1)) O[it] = M::mfma(cf[q], fp[part][it], O[it], x);
             }
             if (q < TILES) {
-                if (two) {
+                if (cuts) {
+#pragma unroll
+                    for (int r = 0; r < AR; ++r) S[q][r] = 0.f;
+                } else if (two) {
 #pragma unroll
                     for (int r = 0; r < AR; ++r) S[q][r] = __builtin_fmaf(S[q][r], ch, S[q][r] * cl);
                 } else {
@@ -618,7 +628,7 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, TS, DA, NW>::MIN_WAVES))
         if (tid == 0 && c0 == 0) {
             const int steps = max(0, min(n, (c_first + seg_chunks) * CH) - c_first * CH);
             const double f = exp((double)gl * steps);
-            J.carry[2 * at] = cut_any ? 0.f : (float)f;
+            J.carry[2 * at] = cut_any ? -1.f : (float)f;
             J.carry[2 * at + 1] = cut_any ? 0.f : (float)(f - (double)(float)f);
         }
     } else if (J.s_out && p.n_seg == 1) {
