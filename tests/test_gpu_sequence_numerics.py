@@ -1,4 +1,6 @@
 """Numerics of the sequence-policy operators that a bound on random values does not see: cases whose sums are exact in f32."""
+import math
+
 import pytest
 import torch
 
@@ -127,3 +129,35 @@ def test_linattn_overflow_of_one_episode_stays_in_it(ops, T, at, d, dtype):
         assert torch.equal(got[n][at + 5:], want[n][at + 5:]), n
     assert torch.equal(got["state_out"], want["state_out"])
     assert not torch.isfinite(got["out"][at:at + 5].float()).all()
+
+
+def test_linattn_step_decay_is_rounded_once(ops):
+    """S exp(log_decay) is the f32 next to its value: long memories (1 - 1e-6 a step) and short ones.  The two floats of the decay are off by 2^-49
+    of it, which the bound on half a step leaves room for."""
+    H, d = 8, 64
+    ld = torch.tensor([-1e-6, -2e-6, -2e-8, -1e-4, -0.01, -0.5, -3.0, -20.0])
+    S = torch.randn(5, H, d, d, generator=gen(1))
+    zero, out, after = torch.zeros(5, H, d, device="cuda"), torch.empty(5, H, d, device="cuda"), torch.empty(5, H, d, d, device="cuda")
+    ops.linattn_step(zero, zero, zero, out, ld.cuda(), S.cuda(), state_out=after)
+    want = S.double() * torch.exp(ld.double()).view(1, H, 1, 1)
+    half = torch.ldexp(torch.ones_like(want), torch.frexp(want).exponent - 25)
+    assert ((after.cpu().double() - want).abs() <= half * (1 + 2.0 ** -20)).all()
+
+
+def test_linattn_step_and_sequence_agree_on_decays_at_both_ends(ops):
+    """No decay, positive (taken as 0), no memory, NaN: what the sequence form makes of them."""
+    ld = torch.tensor([0.0, 0.5, -math.inf, math.nan, -1.0])
+    g = gen(2)
+    q, k, v = (torch.randn(1, 2, 5, 16, generator=g).cuda() for _ in range(3))
+    S = torch.randn(2, 5, 16, 16, generator=g).cuda()
+    a, b, o1, o2 = torch.empty_like(S), torch.empty_like(S), torch.empty_like(v), torch.empty_like(v)
+    ops.linattn_forward(q, k, v, o1, ld.cuda(), state=S, state_out=a)
+    ops.linattn_step(q[0], k[0], v[0], o2[0], ld.cuda(), S, state_out=b)
+    for t in (o1[0], o2[0], a, b):
+        assert torch.isnan(t[:, 3]).all()
+    rest = [0, 1, 2, 4]
+    # 16 products and sums, three roundings of a state: under 64 u of the terms' magnitudes
+    lam = torch.exp(ld.clamp(max=0.0)).view(1, 5, 1, 1).cuda()
+    mag = (lam * S.abs() + k[0, ..., :, None].abs() * v[0, ..., None, :].abs())[:, rest]
+    assert ((a[:, rest] - b[:, rest]).abs() <= 8 * 2.0 ** -24 * mag).all()
+    assert ((o1[0][:, rest] - o2[0][:, rest]).abs() <= 64 * 2.0 ** -24 * (q[0][:, rest].abs()[..., None] * mag).sum(2)).all()

@@ -59,7 +59,10 @@ __global__ void __launch_bounds__(256) linattn_step_kernel(xrl_linattn_t p) {
     const int bh = blockIdx.x, b = bh / p.H, h = bh % p.H;
     const int nc = (p.dv + 3) >> 2, groups = blockDim.x / nc;
     const int c4 = threadIdx.x % nc, g = threadIdx.x / nc;
-    const float lam = expf(fminf(p.log_decay[h], 0.f));
+    // the decay as two floats, as in the sequence form: of a long memory one alone is off by a fair part of what it forgets (-1e-6: 1.3 %)
+    const float gl = p.log_decay[h];
+    const double decay = exp((double)(gl > 0.f ? 0.f : gl < -1e30f ? -1e30f : gl));
+    const float lam = (float)decay, lam_low = (float)(decay - (double)lam);
     const bool cut = p.reset && p.reset[b] != 0.f;
     const E* q = (const E*)p.q + b * p.stride_q[1] + h * p.stride_q[2];
     const E* k = (const E*)p.k + b * p.stride_k[1] + h * p.stride_k[2];
@@ -80,7 +83,10 @@ __global__ void __launch_bounds__(256) linattn_step_kernel(xrl_linattn_t p) {
             }
             const float kd = io_load(k + d), qd = io_load(q + d);
 #pragma unroll
-            for (int m = 0; m < 4; ++m) { s[m] = lam * s[m] + kd * vv[m]; acc[m] += qd * s[m]; }
+            for (int m = 0; m < 4; ++m) {
+                s[m] = __builtin_fmaf(s[m], lam, __builtin_fmaf(s[m], lam_low, kd * vv[m]));
+                acc[m] += qd * s[m];
+            }
             if (VEC) *reinterpret_cast<f32x4_t*>(p.state_out + at) = s;
             else
 #pragma unroll
