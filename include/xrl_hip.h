@@ -1603,7 +1603,7 @@ typedef struct {
     int64_t N, ld, ld_d;
     int32_t A, K;                  /* K in 1..256 */
     int32_t dtype;
-    float temperature, grad_scale; int32_t pad;
+    float temperature, grad_scale; int32_t pad;   /* temperature: 1e-18..1e18, so that its square and reciprocal are numbers */
 } xrl_distill_t;
 int xrl_distill_loss(const xrl_distill_t* p, xrl_stream_t stream);
 

@@ -594,7 +594,7 @@ extern "C" int xrl_distill_loss(const xrl_distill_t* pp, xrl_stream_t stream) {
     XRL_CHECK_ARG(pp != nullptr);
     const xrl_distill_t& p = *pp;
     XRL_CHECK_ARG(p.N >= 0 && p.N <= 0x7fffffff && p.A >= 1 && p.A <= 1 << 30 && p.K >= 1 && p.K <= DISTILL_MAX_K);
-    XRL_CHECK_ARG((p.dtype == XRL_F32 || p.dtype == XRL_BF16) && p.temperature > 0.f);
+    XRL_CHECK_ARG((p.dtype == XRL_F32 || p.dtype == XRL_BF16) && p.temperature >= 1e-18f && p.temperature <= 1e18f);
     if (p.N == 0) return XRL_OK;
     XRL_CHECK_ARG(p.logits && p.teacher_idx && p.teacher_logits && p.loss);
     const int e = p.dtype == XRL_F32 ? 4 : 2;

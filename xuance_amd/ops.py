@@ -1431,8 +1431,8 @@ def distill_loss(logits, teacher_idx, teacher_logits, loss, d_logits=None, avail
         loss_n = weight_n tau^2 KL(softmax(teacher_logits_n / tau) || softmax(logits_n / tau) at teacher_idx_n)     [N] float32
         d_logits = grad_scale * d(sum loss) / d logits
     logits, d_logits [N, A] float32 or bfloat16 with rows of any stride (d_logits may be logits), teacher_idx [N, K] int32 (outside 0..A-1:
-    no entry), teacher_logits [N, K] of the type of logits, K up to 256, avail [N, A] float32 0/1, weight [N] float32.  A row without a
-    valid teacher entry, without an available logit or of weight 0 has loss 0 and gradient 0."""
+    no entry), teacher_logits [N, K] of the type of logits, K up to 256, avail [N, A] float32 0/1, weight [N] float32, temperature 1e-18 to
+    1e18.  A row without a valid teacher entry, without an available logit or of weight 0 has loss 0 and gradient 0."""
     if logits.dim() != 2 or teacher_idx.dim() != 2:
         raise XrlError("logits: [N, A], teacher_idx: [N, K]")
     dev, typ, f32, i32 = torch.cuda.current_device(), logits.dtype, torch.float32, torch.int32
