@@ -1546,7 +1546,7 @@ typedef struct {
     float* workspace;        /* xrl_linattn_workspace_floats() floats, 16-byte aligned; contents need not survive the call */
     int64_t workspace_floats;
     int64_t stride_q[3], stride_k[3], stride_v[3], stride_out[3], stride_d_out[3], stride_d_q[3], stride_d_k[3], stride_d_v[3];
-    int32_t T, B, H, dk, dv; /* dk, dv in 1..128 */
+    int32_t T, B, H, dk, dv; /* dk, dv in 1..128; B * H up to 2^24; whole sequences: 64 to 1536 threads for each of them, under 2^32 in all */
     int32_t dtype;           /* XRL_F32, XRL_BF16: q k v out and their gradients */
     float scale; int32_t pad;
 } xrl_linattn_t;

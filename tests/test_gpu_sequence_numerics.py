@@ -161,3 +161,19 @@ def test_linattn_step_and_sequence_agree_on_decays_at_both_ends(ops):
     mag = (lam * S.abs() + k[0, ..., :, None].abs() * v[0, ..., None, :].abs())[:, rest]
     assert ((a[:, rest] - b[:, rest]).abs() <= 8 * 2.0 ** -24 * mag).all()
     assert ((o1[0][:, rest] - o2[0][:, rest]).abs() <= 64 * 2.0 ** -24 * (q[0][:, rest].abs()[..., None] * mag).sum(2)).all()
+
+
+def test_linattn_step_of_many_rows(ops):
+    """16.8 million rows and heads, each with 256 threads: more than a launch takes."""
+    B, H = 1 << 22, 4
+    g = torch.Generator(device="cuda")
+    g.manual_seed(3)
+    q, k, v = (torch.randn(B, H, 2, generator=g, device="cuda") for _ in range(3))
+    S, out, reset = torch.randn(B, H, 2, 2, generator=g, device="cuda"), torch.empty(B, H, 2, device="cuda"), (torch.rand(B, generator=g, device="cuda") < 0.5).float()
+    ld = torch.tensor([-0.1, -0.2, -0.3, -0.4], device="cuda")
+    after = torch.full_like(S, 7.5)
+    ops.linattn_step(q, k, v, out, ld, S, state_out=after, reset=reset)
+    for rows in (slice(0, 1000), slice((1 << 21) - 500, (1 << 21) + 500), slice(B - 1000, B)):
+        o, a = torch.empty(1000, H, 2, device="cuda"), torch.empty(1000, H, 2, 2, device="cuda")
+        ops.linattn_step(q[rows], k[rows], v[rows], o, ld, S[rows], state_out=a, reset=reset[rows])
+        assert torch.equal(out[rows], o) and torch.equal(after[rows], a)

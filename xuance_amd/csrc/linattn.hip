@@ -291,14 +291,27 @@ extern "C" int xrl_linattn_step(const xrl_linattn_t* pp, xrl_stream_t stream) {
     if (int rc = check_tensors(p, false)) return rc;
     const bool vec = p.dv % 4 == 0 && ((reinterpret_cast<uintptr_t>(p.state) | reinterpret_cast<uintptr_t>(p.state_out)) & 15) == 0;
     const int threads = 256;
-    const dim3 grid(p.B * p.H);
-    if (p.dtype == XRL_F32) {
-        if (vec) hipLaunchKernelGGL((linattn_step_kernel<float, true>), grid, dim3(threads), 0, as_stream(stream), p);
-        else hipLaunchKernelGGL((linattn_step_kernel<float, false>), grid, dim3(threads), 0, as_stream(stream), p);
-    } else {
-        if (vec) hipLaunchKernelGGL((linattn_step_kernel<bf16_t, true>), grid, dim3(threads), 0, as_stream(stream), p);
-        else hipLaunchKernelGGL((linattn_step_kernel<bf16_t, false>), grid, dim3(threads), 0, as_stream(stream), p);
+    const int64_t most = p.H < 1 << 23 ? (1 << 23) / p.H : 1, e = p.dtype == XRL_F32 ? 4 : 2;       // rows of a launch, which takes under 2^32 threads
+    XRL_CHECK_ARG(p.H < 1 << 24);
+    for (int64_t first = 0; first < p.B; first += most) {
+        xrl_linattn_t r = p;
+        r.B = (int)(p.B - first < most ? p.B - first : most);
+        r.q = (const char*)p.q + first * p.stride_q[1] * e;
+        r.k = (const char*)p.k + first * p.stride_k[1] * e;
+        r.v = (const char*)p.v + first * p.stride_v[1] * e;
+        r.out = (char*)p.out + first * p.stride_out[1] * e;
+        r.state = p.state + first * p.H * p.dk * p.dv;
+        r.state_out = p.state_out + first * p.H * p.dk * p.dv;
+        if (p.reset) r.reset = p.reset + first;
+        const dim3 grid(r.B * r.H);
+        if (p.dtype == XRL_F32) {
+            if (vec) hipLaunchKernelGGL((linattn_step_kernel<float, true>), grid, dim3(threads), 0, as_stream(stream), r);
+            else hipLaunchKernelGGL((linattn_step_kernel<float, false>), grid, dim3(threads), 0, as_stream(stream), r);
+        } else {
+            if (vec) hipLaunchKernelGGL((linattn_step_kernel<bf16_t, true>), grid, dim3(threads), 0, as_stream(stream), r);
+            else hipLaunchKernelGGL((linattn_step_kernel<bf16_t, false>), grid, dim3(threads), 0, as_stream(stream), r);
+        }
+        XRL_CHECK_LAUNCH();
     }
-    XRL_CHECK_LAUNCH();
     return XRL_OK;
 }

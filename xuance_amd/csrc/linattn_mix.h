@@ -649,7 +649,7 @@ static int launch_mix_as(mix_t m, int dc, hipStream_t s) {
     static_assert(G::BYTES + 1500 <= 160 * 1024, "LDS");
     m.n_slices = (dc + G::DC - 1) / G::DC;
     const int64_t units = ((int64_t)m.B * m.H * m.n_seg + 7) / 8 * 8, grid = units * m.n_jobs * m.n_slices;
-    XRL_CHECK_ARG(grid <= 0x7fffffff);
+    XRL_CHECK_ARG(grid * G::NT < 1ll << 32);                         // threads of a launch
     hipLaunchKernelGGL((linattn_mix_kernel<E, TS, DA, NW, FULL>), dim3((unsigned)grid), dim3(64 * NW), G::BYTES, s, m);
     XRL_CHECK_LAUNCH();
     return XRL_OK;
