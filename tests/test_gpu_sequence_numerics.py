@@ -177,3 +177,33 @@ def test_linattn_step_of_many_rows(ops):
         o, a = torch.empty(1000, H, 2, device="cuda"), torch.empty(1000, H, 2, 2, device="cuda")
         ops.linattn_step(q[rows], k[rows], v[rows], o, ld, S[rows], state_out=a, reset=reset[rows])
         assert torch.equal(out[rows], o) and torch.equal(after[rows], a)
+
+
+# ------------------------------------------------------------------------------------------------------- distillation
+def test_distill_of_many_rows(ops):
+    """537 million rows, 8 threads each: more than a launch takes.  The policy's logits are one row for all."""
+    N = (1 << 29) + 5
+    logits = torch.tensor([[0.5, -1.0]], device="cuda").expand(N, 2)
+    idx, top, loss = torch.ones(N, 1, dtype=torch.int32, device="cuda"), torch.zeros(N, 1, device="cuda"), torch.full((N,), 7.5, device="cuda")
+    idx[-3:] = 0
+    ops.distill_loss(logits, idx, top, loss)
+    want = math.log(1 + math.exp(1.5)), math.log(1 + math.exp(-1.5))
+    for part, ref in ((loss[:-3], want[0]), (loss[-3:], want[1])):
+        assert part.max() == part.min() and abs(part[0].item() - ref) <= 16 * 2.0 ** -24 * (ref + 1.5)
+
+
+def test_distill_rows_of_several_launches(ops):
+    """Every tensor of a call goes on at the right row."""
+    N, A, K = (1 << 21) + 77, 3, 2
+    g = torch.Generator(device="cuda")
+    g.manual_seed(4)
+    logits, top = torch.randn(N, A, generator=g, device="cuda"), torch.randn(N, K, generator=g, device="cuda")
+    idx = torch.randint(0, A, (N, K), generator=g, device="cuda", dtype=torch.int32)
+    avail, weight = (torch.rand(N, A, generator=g, device="cuda") < 0.7).float(), torch.rand(N, generator=g, device="cuda")
+    wide = torch.full((N, A + 2), 7.5, device="cuda")
+    loss, d = torch.full((N,), 7.5, device="cuda"), wide[:, 1:-1]
+    ops.distill_loss(logits, idx, top, loss, d_logits=d, avail=avail, weight=weight)
+    rows = slice((1 << 21) - 100, N)
+    l2, d2 = torch.empty(177, device="cuda"), torch.empty(177, A, device="cuda")
+    ops.distill_loss(logits[rows], idx[rows], top[rows], l2, d_logits=d2, avail=avail[rows], weight=weight[rows])
+    assert torch.equal(loss[rows], l2) and torch.equal(d[rows], d2) and (wide[:, 0] == 7.5).all() and (wide[:, -1] == 7.5).all()

@@ -604,8 +604,20 @@ extern "C" int xrl_distill_loss(const xrl_distill_t* pp, xrl_stream_t stream) {
                        {"weight", p.weight, 4, 1, {p.N}, {1}, false}};
     const int pairs[][2] = {{0, 2}};
     if (int rc = check_args(a, 7, pairs, 1)) return rc;
-    if (p.dtype == XRL_F32) launch_distill<float>(p, as_stream(stream));
-    else launch_distill<bf16_t>(p, as_stream(stream));
-    XRL_CHECK_LAUNCH();
+    // a launch takes under 2^32 threads, and a row 1024 of them at most
+    for (int64_t first = 0; first < p.N; first += 1 << 21) {
+        xrl_distill_t r = p;
+        r.N = p.N - first < 1 << 21 ? p.N - first : 1 << 21;
+        r.logits = (const char*)p.logits + first * p.ld * e;
+        r.teacher_idx = p.teacher_idx + first * p.K;
+        r.teacher_logits = (const char*)p.teacher_logits + first * p.K * e;
+        if (p.avail) r.avail = p.avail + first * p.A;
+        if (p.weight) r.weight = p.weight + first;
+        r.loss = p.loss + first;
+        if (p.d_logits) r.d_logits = (char*)p.d_logits + first * p.ld_d * e;
+        if (p.dtype == XRL_F32) launch_distill<float>(r, as_stream(stream));
+        else launch_distill<bf16_t>(r, as_stream(stream));
+        XRL_CHECK_LAUNCH();
+    }
     return XRL_OK;
 }
