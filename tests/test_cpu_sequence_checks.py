@@ -1,8 +1,11 @@
 """More of what the host side of the sequence-policy operators refuses (nothing is launched)."""
 import math
+import subprocess
+import sys
 
 import pytest
 
+from conftest import ROOT
 from test_cpu_sequence_ops import call, filled, lin
 
 
@@ -23,3 +26,11 @@ def test_linattn_refuses_more_threads_than_a_launch_takes(entry):
     strides = {"stride_" + n: (1 << 30, 64, 64) for n in ("q", "k", "v", "out", "d_out", "d_q", "d_k", "d_v")}
     assert call(entry, lin(T=1, B=1 << 24, H=1, dk=64, dv=64, **far, **strides)) == -1
     assert b"1ll << 32" in _lib.load().xrl_last_error()
+
+
+def test_ops_import_without_device_bindings():
+    """A torch built for the CPU alone has no raw-stream binding: the package's modules import all the same."""
+    src = ("import torch, sys\nif hasattr(torch._C, '_cuda_getCurrentRawStream'): del torch._C._cuda_getCurrentRawStream\n"
+           f"sys.path.insert(0, {ROOT!r})\nimport xuance_amd.ops\n")
+    r = subprocess.run([sys.executable, "-c", src], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr[-500:]

@@ -1226,7 +1226,7 @@ def _need(cond, what):
         raise XrlError(what)
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)           # a torch without device bindings has none, and no calls of it
 
 
 def _explain(device, *tensors):
