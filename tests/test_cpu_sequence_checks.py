@@ -4,6 +4,7 @@ import subprocess
 import sys
 
 import pytest
+import torch
 
 from conftest import ROOT
 from test_cpu_sequence_ops import call, filled, lin
@@ -34,3 +35,12 @@ def test_ops_import_without_device_bindings():
            f"sys.path.insert(0, {ROOT!r})\nimport xuance_amd.ops\n")
     r = subprocess.run([sys.executable, "-c", src], capture_output=True, text=True)
     assert r.returncode == 0, r.stderr[-500:]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float64, torch.int32])
+def test_workspace_sizes_refuse_other_types(dtype):
+    from xuance_amd import ops
+    with pytest.raises(ops.XrlError):
+        ops.linattn_workspace_floats(100, 1, 1, 8, 8, dtype=dtype)
+    with pytest.raises(ops.XrlError):
+        ops.block_norm_workspace_floats(100, 8, dtype=dtype)

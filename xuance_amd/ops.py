@@ -1245,9 +1245,13 @@ def _explain(device, *tensors):
             raise XrlError(f"{name}: its last dimension has to be contiguous, strides are {t.stride()}")
 
 
+def _io_code(dtype):
+    _need(dtype in _IO_DTYPES, f"float32 or bfloat16 activations, got {dtype}")
+    return _IO_DTYPES[dtype]
+
+
 def _io_dtype(t):
-    _need(t.dtype in _IO_DTYPES, f"float32 or bfloat16 activations, got {t.dtype}")
-    return _IO_DTYPES[t.dtype]
+    return _io_code(t.dtype)
 
 
 def _workspace(given, floats, device):
@@ -1264,7 +1268,7 @@ def _workspace(given, floats, device):
 
 def linattn_workspace_floats(T, B, H, dk, dv, backward=False, dtype=torch.float32):
     """Floats of workspace that linattn_forward / linattn_backward need at these sizes (0: none)."""
-    p = _LINATTN.pack(*(0,) * 41, int(T), int(B), int(H), int(dk), int(dv), _IO_DTYPES[dtype], 1.0, 0)
+    p = _LINATTN.pack(*(0,) * 41, int(T), int(B), int(H), int(dk), int(dv), _io_code(dtype), 1.0, 0)
     n = _lib.load().xrl_linattn_workspace_floats(p, int(bool(backward)))
     _lib.check(min(n, 0), "xrl_linattn_workspace_floats")
     return n
@@ -1398,7 +1402,7 @@ def block_norm_forward(x, u, y, n=None, gate=None, gate_act="sigmoid", scale=Non
 
 def block_norm_workspace_floats(N, D, dtype=torch.float32):
     """Floats of workspace that block_norm_backward needs for N rows of D values."""
-    n = _lib.load().xrl_block_norm_workspace_floats(_BLOCK_NORM.pack(*(0,) * 22, int(N), *(0,) * 10, int(D), _IO_DTYPES[dtype], 0, 0, 1e-5, 0))
+    n = _lib.load().xrl_block_norm_workspace_floats(_BLOCK_NORM.pack(*(0,) * 22, int(N), *(0,) * 10, int(D), _io_code(dtype), 0, 0, 1e-5, 0))
     _lib.check(min(n, 0), "xrl_block_norm_workspace_floats")
     return n
 
