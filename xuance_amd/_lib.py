@@ -413,6 +413,12 @@ class Distill(C.Structure):
                 ("dtype", c_int32), ("temperature", c_float), ("grad_scale", c_float), ("pad", c_int32)]
 
 
+def pack_format(cls):
+    """The struct module's format of these fields, for callers that pack a whole struct at once."""
+    codes = {c_void_p: "P", c_int64: "q", c_int32: "i", c_float: "f"}
+    return "@" + "".join(f"{t._length_}{codes[t._type_]}" if hasattr(t, "_length_") else codes[t] for _, t in cls._fields_)
+
+
 _SIGS = {
     "xrl_linattn_forward": [c_void_p, c_void_p],
     "xrl_linattn_backward": [c_void_p, c_void_p],

@@ -1212,11 +1212,9 @@ def gru_backward(**kw):
 
 
 # ------------------------------------------------------------------------------------------ sequence policies
-# The structs are packed in one go (their layouts: _lib.LinAttn, BlockNorm, Distill): an acting step is a launch of microseconds, and setting
-# fifty ctypes fields one by one takes as long.
-_LINATTN = struct.Struct("@16Pq24q6ifi")
-_BLOCK_NORM = struct.Struct("@21P12q4ifi")
-_DISTILL = struct.Struct("@7P3q3iffi")
+# The structs are packed in one go, in the order of their fields: an acting step is a launch of microseconds, and setting fifty ctypes fields one by
+# one takes as long.
+_LINATTN, _BLOCK_NORM, _DISTILL = (struct.Struct(_lib.pack_format(cls)) for cls in (_lib.LinAttn, _lib.BlockNorm, _lib.Distill))
 _IO_DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 NORM_KIND = {"rms": 0, "layer": 1}
 
