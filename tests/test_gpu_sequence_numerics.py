@@ -1,8 +1,13 @@
-"""Numerics of the sequence-policy operators that a bound on random values does not see: cases whose sums are exact in f32."""
+"""Numerics of the sequence-policy operators: cases whose sums are exact in f32, what is not finite, sizes beyond a launch, and random values against
+bounds of the kernels' own roundings (tests/sequence_bounds.py; tests/test_cpu_sequence_bounds.py plants mistakes that these have to see)."""
 import math
 
 import pytest
 import torch
+
+import sequence_bounds as sb
+from test_cpu_sequence_bounds import DISTILL_SIZES, NORM_SIZES, distill_case, lines_of, norm_case
+from test_gpu_sequence_ops import lin_case, lin_expected, lin_run, lin_terms
 
 pytestmark = pytest.mark.gpu
 
@@ -131,6 +136,24 @@ def test_linattn_overflow_of_one_episode_stays_in_it(ops, T, at, d, dtype):
     assert not torch.isfinite(got["out"][at:at + 5].float()).all()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("T,B,H,dk,dv", [(1500, 4, 1, 128, 128), (1500, 4, 1, 128, 64), (2100, 3, 2, 64, 128), (1100, 5, 1, 32, 32)])
+def test_linattn_split_ragged_rows(ops, T, B, H, dk, dv, dtype):
+    """Rows of several lengths, resets and a state, the time axis cut into segments; and the same bits when it runs again.  An output is held to what
+    f32 sums may be off by in either type, a bf16 one to its own rounding more."""
+    assert ops.linattn_workspace_floats(T, B, H, dk, dv, dtype=dtype) > 0 and ops.linattn_workspace_floats(T, B, H, dk, dv, backward=True, dtype=dtype) > 0
+    c = lin_case(T + dk, T, B, H, dk, dv, dtype, "ragged", False, True, log_decay=[-0.004, -0.1][:H])
+    c["reset"] = torch.zeros(T, B)
+    c["reset"][T // 3, 0] = c["reset"][200, 1] = 1
+    got, again = lin_run(ops, c), lin_run(ops, c)
+    ref, mag = lin_expected(c)
+    rel = lin_terms(dk, dv, T, F32)
+    for n in got:
+        assert torch.equal(got[n], again[n]), n
+        stored = 2.0 ** -8 * (1 + rel) * ref[n].abs() if got[n].dtype is BF16 else 0.0
+        assert ((got[n].cpu().double() - ref[n]).abs() <= rel * mag[n] * (1 + 2.0 ** -8) + stored + 1e-37).all(), n
+
+
 def test_linattn_step_decay_is_rounded_once(ops):
     """S exp(log_decay) is the f32 next to its value: long memories (1 - 1e-6 a step) and short ones.  The two floats of the decay are off by 2^-49
     of it, which the bound on half a step leaves room for."""
@@ -179,6 +202,24 @@ def test_linattn_step_of_many_rows(ops):
         assert torch.equal(out[rows], o) and torch.equal(after[rows], a)
 
 
+# ------------------------------------------------------------------------------------------------------- block norm
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("gate", [True, False], ids=["gate", "open"])
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("N,D", NORM_SIZES)
+def test_block_norm_within_its_roundings(ops, N, D, kind, gate, dtype):
+    c = norm_case(N, D, dtype, gate)
+    dev = {n: (None if t is None else t.cuda()) for n, t in c.items()}
+    par = dict(kind=kind, eps=1e-5, gate_act="sigmoid", **{n: dev[n] for n in ("gate", "scale", "w_post", "b_post", "w_pre", "b_pre")})
+    got = {n: torch.full((N, D), 7.5, device="cuda", dtype=dtype) for n in ("y", "n", "d_x", "d_u") + (("d_gate",) if gate else ())}
+    got.update({n: torch.full((D,), 7.5, device="cuda") for n in ("d_scale", "d_w_post", "d_b_post", "d_w_pre", "d_b_pre")})
+    ops.block_norm_forward(dev["x"], dev["u"], got["y"], got["n"], **par)
+    ops.block_norm_backward(dev["x"], dev["u"], dev["d_y"], dev["d_n"], **{k: v for k, v in got.items() if k.startswith("d_")}, **par)
+    for n, (want, bound) in sb.norm_exact(c, kind, 1e-5, lines_of(N, D, dtype)).items():
+        worst = ((got[n].cpu().double() - want).abs() / bound).max().item()
+        assert worst <= 1, (n, worst)
+
+
 # ------------------------------------------------------------------------------------------------------- distillation
 def test_distill_of_many_rows(ops):
     """537 million rows, 8 threads each: more than a launch takes.  The policy's logits are one row for all."""
@@ -207,3 +248,22 @@ def test_distill_rows_of_several_launches(ops):
     l2, d2 = torch.empty(177, device="cuda"), torch.empty(177, A, device="cuda")
     ops.distill_loss(logits[rows], idx[rows], top[rows], l2, d_logits=d2, avail=avail[rows], weight=weight[rows])
     assert torch.equal(loss[rows], l2) and torch.equal(d[rows], d2) and (wide[:, 0] == 7.5).all() and (wide[:, -1] == 7.5).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("avail", [False, True], ids=["open", "masked"])
+@pytest.mark.parametrize("tau", [2.0, 0.4])
+@pytest.mark.parametrize("N,A,K", DISTILL_SIZES)
+def test_distill_within_its_roundings(ops, N, A, K, tau, avail, dtype):
+    """Loss and gradient, and the loss alone: the same bits."""
+    c = distill_case(N, A, K, dtype, avail)
+    dev = {n: (None if t is None else t.cuda()) for n, t in c.items()}
+    loss, alone, d = torch.full((N,), 7.5, device="cuda"), torch.full((N,), 7.5, device="cuda"), torch.full((N, A), 7.5, device="cuda", dtype=dtype)
+    par = dict(avail=dev["avail"], weight=dev["weight"], temperature=tau, grad_scale=0.5)
+    ops.distill_loss(dev["logits"], dev["teacher_idx"], dev["teacher_logits"], loss, d_logits=d, **par)
+    ops.distill_loss(dev["logits"], dev["teacher_idx"], dev["teacher_logits"], alone, **par)
+    assert torch.equal(loss, alone)
+    want, bound, grad, grad_bound = sb.distill_exact(c, tau, 0.5)
+    for n, g, v, e in (("loss", loss, want, bound), ("d_logits", d, grad, grad_bound)):
+        off = (g.cpu().double() - v).abs()
+        assert (off <= e).all(), (n, (off / e.clamp(min=1e-300)).max().item())
