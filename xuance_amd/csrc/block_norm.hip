@@ -6,8 +6,8 @@
 // pass recomputes p, y and both statistics from the x, u and gate it needs anyway.  A row lives in the registers of L lanes, 8 values
 // each, from its one load to its one store; the gradient sums over the rows stay in registers over all rows of a workgroup, the parameters in LDS.
 // Those sums leave as one line of partials per workgroup and a second launch adds the lines in a fixed order (no atomics).
-// Measured, forward and backward: 65536 x 256 f32 with a gate, rms 65 us (5.2 TB/s) and 103 us (5.2), as a copy; 30011 x 2048 bf16, layer, 142 us
-// (4.3) and 240 us (4.1): a row of 2048 is four waves that meet six times, and the vector instructions of two or three rows a CU do not hide that.
+// Measured, forward and backward with its sums: 65536 x 256 f32 with a gate, rms 64 us (5.2 TB/s) and 110 us (4.9), as a copy; 30011 x 2048 bf16, layer,
+// 131 us (4.7) and 216 us (4.6): a row of 2048 is four waves that meet six times, and the vector instructions of two or three rows a CU do not hide that.
 #include "args.h"
 #include "io16.h"
 #include "lanes.h"
@@ -20,7 +20,8 @@ constexpr int NV = 8;                  // values of a row per lane
 // the memory's time for 16-bit rows.
 __device__ __forceinline__ float fma_f(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
 
-// act_apply_c with the sigmoid from v_exp_f32 and v_rcp_f32 (a unit in the last place each) instead of expf and a division
+// act_apply_c with the sigmoid a from v_exp_f32 and v_rcp_f32 (a unit in the last place each) instead of expf and a division.  The exponential's argument
+// is rounded too, so a is off by up to ((1 - a) (1.5 |z| + 2) + 3) 2^-24 of itself: far out, where a is small, by |z| of its last places.
 template <int ACT>
 __device__ __forceinline__ float gate_act_c(float z) {
     if (ACT == XRL_ACT_SIGMOID) return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * z));
@@ -28,7 +29,7 @@ __device__ __forceinline__ float gate_act_c(float z) {
 }
 // Sums over the rows, with a the activated gate, uhat and yhat the normalised u and y:  S0 = sum a d_y,  S1 = sum a d_y uhat,  S2 = sum d_n yhat,
 // S3 = sum d_n.  They give d_scale = w_post S1 + b_post S0, d_w_post = scale S1, d_b_post = scale S0, d_w_pre = S2, d_b_pre = S3.  (Where w_post uhat
-// and b_post cancel in p, d_scale loses no more than the rounding of uhat costs it anyway.)
+// and b_post cancel in p over all rows, d_scale is off by the roundings of uhat, which p has too, and by those of the two sums.)
 constexpr int NORM_SUMS = 4;
 
 // FULL below: rows of exactly 8 L values, without the checks of a row's end (30011 x 2048 bf16: with the sums by lanes.h 431 -> 386 us)

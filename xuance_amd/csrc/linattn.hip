@@ -169,10 +169,11 @@ static void backward_jobs(const xrl_linattn_t& p, mix_job_t* j) {
 //   + ceil(... states n / slots) (chunks / n + 2) / 2 + 3    for n > 1 the pass over the segments' own states, their joining and two launches,
 //   + rows heads states n dk dv / 2^21                       and the states' way through memory;
 // the cheapest n up to 64 is taken.  Measured, forward / backward in us, * where the rule goes:
-//   8 rows, 8 heads, 4096 steps, 128 wide, bf16:    n = 1 302 / 316,  4 146 / 318,  8 138* / 333*,  16 169 / 375
-//   1 row, 8 heads, 32768 steps, 128 wide, bf16:    16 251 / 351,  32 151 / 313 (21: 307*),  64 137* / 336,  128 163 / 392
-//   2 rows, 4 heads, 8192 steps, 64 wide, f32:      1 708 / 714,  8 138 / 143,  16 78 / 111 (21: 110*),  32 53* / 96
-//   16 rows, 8 heads, 1024 steps, 128 wide, bf16:   1 83 / 118*,  2 89 / 181,  4 84* / 196
+//   8 rows, 8 heads, 4096 steps, 128 wide, bf16:    n = 1 367 / 379,  4 162 / 359,  8 153* / 371*,  16 176 / 404
+//   1 row, 8 heads, 32768 steps, 128 wide, bf16:    16 281 / 389,  32 171 / 363 (21: 353*),  64 155* / 376,  128 182 / 426
+//   2 rows, 4 heads, 8192 steps, 64 wide, f32:      1 719 / 724,  8 141 / 147,  16 80 / 112,  32 54* / 93*
+//   16 rows, 8 heads, 1024 steps, 128 wide, bf16:   1 98 / 145*,  2 100 / 198,  4 92* / 212
+// Backward the rule is up to 3 % from the best of these: a compute unit's second workgroup gains less than the rule's slots say.
 static int segments(const xrl_linattn_t& p, int n_jobs) {
     const int64_t units = (int64_t)p.B * p.H, wide = p.dk > p.dv ? p.dk : p.dv, da = n_jobs > 1 ? wide : p.dk, dc = n_jobs > 1 ? wide : p.dv;
     const int chunks = (p.T + CH - 1) / CH, states = n_jobs > 1 ? 2 : 1;

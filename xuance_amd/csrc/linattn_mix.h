@@ -15,10 +15,12 @@
 // computes what f32 sums make of its inputs, and a bf16 result is rounded once, where it is stored.  Powers of lam are made in f64; lam^64, applied
 // to the state at every chunk, keeps its rounding error as a second float.
 //
-// Bound.  f32: the matrix instructions (half of a large product's rate): 256 rows x 256 steps, 4 heads of 64: 98 us forward, 280 us the three gradients.
-// bf16, heads of 128: a chunk takes a compute unit 9.7 k cycles, 27% of them matrix instructions, 36% vector instructions (two-part operands, decays),
-// 38% LDS, one after another in the two workgroups that registers and LDS allow; 8 ragged rows x 4096 steps, 8 heads: 80 us forward, 200 us the gradients,
-// the passes over segment states not counted.
+// Bound.  f32: the matrix instructions (half of a large product's rate): 256 rows x 256 steps, 4 heads of 64: 91 us forward, 229 us the three gradients,
+// in a run of hundreds of passes (the first 20 after a pause take a fifth more).
+// bf16, heads of 128: a chunk takes a compute unit 10.9 k cycles, 35% of them matrix instructions, 46% vector instructions (three-part operands, decays),
+// 35% LDS, mostly one after another in the two workgroups that registers and LDS allow; 8 ragged rows x 4096 steps, 8 heads: 77 us forward and 35 + 16 us for
+// the states of its segments and their joining, 220 us and 66 + 29 us the gradients.  (With two-part operands, 17 bits of them, 9.7 k cycles a chunk; in turn on one
+// card: this case 373 us with two, 429 with three.)
 #pragma once
 #include "io16.h"
 
@@ -259,7 +261,7 @@ struct mix_geom {
     static constexpr int DC = TS * NW, NT = 64 * NW, SA = DA + M::PAD_A, SB = DA + M::PAD_B, SC = DC + M::PAD_C, SP = CH + M::PAD_P;
     static constexpr int P_SIZE = M::P_PARTS * CH * SP, P_TILES = (CH / TS) * (CH / TS + 1) / 2, MINE = (P_TILES + NW - 1) / NW;
     // P in the place of A, which costs a barrier, where a wave's tiles of P fit its registers and a third workgroup fits the compute unit for it:
-    // 256 rows of 256 steps, 4 heads of 64, f32, forward and backward 387 us with two workgroups, 370 with three
+    // 256 rows of 256 steps, 4 heads of 64, f32, forward and backward 349 us with two workgroups, 319 with three
     static constexpr int OTHER = 1280, OVER_SIZE = P_SIZE > CH * SA ? P_SIZE : CH * SA;
     static constexpr bool OVER = M::KB == TS && MINE <= 3 && 160 * 1024 / up((CH * (SA + SB + SC) + P_SIZE) * (int)sizeof(E) + OTHER) == 2 &&
                                  160 * 1024 / up((OVER_SIZE + CH * (SB + SC)) * (int)sizeof(E) + OTHER) == 3;
@@ -310,7 +312,7 @@ __global__ void __launch_bounds__(64 * NW, (mix_geom<E, TS, DA, NW>::MIN_WAVES))
     typedef const __attribute__((address_space(4))) int* scalar_int_t;
     int b = nth;
     if (p.lengths && p.B <= 64) {
-        // few rows: the longest first, so that the last workgroups to end are short ones (8 ragged rows of 4096 steps, forward and backward, 432 -> 418 us;
+        // few rows: the longest first, so that the last workgroups to end are short ones (8 ragged rows of 4096 steps, forward and backward, 433 -> 411 us;
         // more rows even out by themselves)
         const int mine = lane < p.B ? min(max(p.lengths[lane], 0), p.T) : -1;
         int longer = 0;
